@@ -274,6 +274,72 @@ int q38_spec_step_graph(q38_handle* h, int32_t* position, int32_t* index, int32_
  * silently wrong ids or positions. Reads back one int: a synchronisation of `stream`. */
 int q38_step_status(q38_handle* h, int* status, int clear, void* stream);
 
+/* ---- A key/value cache in pages of 8-bit values, with no counterpart in the reference (its caches are one slab per row, in
+ * bf16 or with a checkpoint's static scales). One q38_paged_cache is one layer's. A page holds page_size positions of every KV
+ * head: keys e4m3 [pages][kv_heads][page_size][head_dim], values e4m3 [pages][kv_heads][page_size / 16][head_dim][16], each
+ * times 2^(b - 127) with b the page's and head's byte of k_scale, v_scale [pages][kv_heads]. head_dim 64, 128 or 256, page_size
+ * 16, 32, 64 or 128; keys and values 16-byte aligned. No initial contents are needed. */
+typedef struct q38_paged_cache {
+    uint8_t *k, *v, *k_scale, *v_scale;
+    int pages, kv_heads, head_dim, page_size;
+} q38_paged_cache;
+
+/* The rows (sequences) of a call and their tokens, side by side in the call's token arrays: row r's are q_start[r] ..
+ * q_start[r + 1] - 1 (int32 [rows + 1] on the device, not falling; from q_start[rows] on tokens belong to no row and are left
+ * alone), or with q_start null max_tokens each. max_tokens bounds every row's tokens (of a row with more the first max_tokens
+ * are taken). position int32 [rows]: the first token's position in its row; negative skips the row (nothing is appended, its
+ * outputs are zero). pages int32 [rows][max_pages]: the pages of each row's positions in order. An entry outside [0, pages), like
+ * a position past the table, names no page: nothing is appended there, and a query that sees it answers NaN. Rows may share
+ * pages that none of them appends to. */
+typedef struct q38_paged_rows {
+    const int32_t *position, *pages, *q_start;
+    int rows, max_pages, tokens, max_tokens;
+} q38_paged_rows;
+
+/* The tokens to append: keys, values and optionally queries (q null: none), bf16, token t's head h at t * *_token + h * *_head
+ * elements (multiples of 4; the pointers 8-byte aligned), its head_dim elements side by side. Queries and keys are RMS-normed
+ * per head where q_norm, k_norm (bf16 [head_dim], used as 1 + w; null: no norm) say so, then their first rotary_dim dims (a
+ * multiple of 8 up to head_dim; 0: no rotation) are rotated, d with d + rotary_dim / 2, by cos, sin bf16 [tokens][rotary_dim]; all
+ * in float32. q_out bf16 [tokens][q_heads][head_dim] receives the queries, of the tokens of every row. */
+typedef struct q38_paged_tokens {
+    const uint16_t *k, *v, *q;
+    uint16_t* q_out;
+    long long k_token, k_head, v_token, v_head, q_token, q_head;
+    int q_heads, rotary_dim;
+    const uint16_t *cos, *sin, *q_norm, *k_norm;
+    float eps;
+} q38_paged_tokens;
+
+/* Append each row's tokens at position .. in its pages. A page's scale is the smallest power of two with every value within
+ * +-448 of it: a page written from its first position on starts anew; one that goes on keeps its scale unless a new value
+ * needs a larger one, and then the positions before the new ones are coded again (a shorter position than before takes tokens
+ * back: they are overwritten, the scale stays). Values are rounded to nearest even. A token whose key or value is not finite in
+ * some head is stored there as a NaN key and a zero value, and leaves the scales alone. No two rows of a call may append to the
+ * same page. */
+int q38_paged_append(const q38_paged_cache* cache, const q38_paged_rows* rows, const q38_paged_tokens* tokens, void* stream);
+
+/* Queries and options of q38_paged_attention: q, out bf16 [tokens][q_heads][head_dim] (16-byte aligned; query head h reads KV
+ * head h / (q_heads / kv_heads), at most 64 to one). The score of position j for the token at position i is scale * q . k_j, then
+ * with cap > 0 cap * tanh(score / cap), then with slopes (float32 [q_heads]) + slope * (j - i). The token sees the positions up
+ * to its own, of them with window > 0 the last `window`; with prefix (int32 [rows]) also those below prefix[row], later tokens of
+ * the call included. A window and a prefix exclude each other. */
+typedef struct q38_paged_query {
+    const uint16_t* q;
+    uint16_t* out;
+    int q_heads;
+    float scale, cap;
+    int window;
+    const float* slopes;
+    const int32_t* prefix;
+} q38_paged_query;
+
+/* Attention of every row's tokens, at positions position .., over its cached positions, the tokens' own (appended before)
+ * among them: softmax over the positions a token sees, float32 sums. scratch holds at least q38_paged_attention_scratch bytes
+ * (256-byte aligned, contents free; null if that is 0); calls that share it must not overlap. */
+int q38_paged_attention(const q38_paged_cache* cache, const q38_paged_rows* rows, const q38_paged_query* query, void* scratch,
+                        size_t scratch_bytes, void* stream);
+size_t q38_paged_attention_scratch(const q38_paged_cache* cache, const q38_paged_rows* rows, int q_heads);
+
 /* Measurement hook, with no counterpart in the reference (for benchmarks that time one kernel inside the step):
  * on != 0 starts bracketing every gate/up projection GEMM launched by q38_verify, q38_mtp_step and q38_spec_step with
  * HIP events on the launch's stream (at most 4096 launches); on == 0 stops, waits for the last event and reports the

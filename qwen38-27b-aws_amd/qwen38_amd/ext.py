@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 from pathlib import Path
+from typing import NamedTuple
 
 import torch
 
@@ -19,7 +20,7 @@ MAX_LAYERS = 128
 EXPORTS = (
     "q38_last_error", "q38_create", "q38_destroy", "q38_buffer_size", "q38_bind", "q38_parity", "q38_set_parity",
     "q38_pack_weight", "q38_pack_weight_fp4", "q38_mxfp4_linear", "q38_fp4_linear", "q38_fp4_linear_scratch", "q38_fp8_linear", "q38_fp8_linear_scratch", "q38_fp8_linear_f32", "q38_fp8_linear_mfma", "q38_fp8_linear_noalloc", "q38_mlp_up", "q38_tiles_size", "q38_verify", "q38_decode", "q38_copy_states", "q38_prefill", "q38_mtp_prefill", "q38_mtp_step", "q38_head_groupmax", "q38_head_pick", "q38_embed", "q38_accept", "q38_spec_step", "q38_spec_step_graph", "q38_verify_step", "q38_step_status",
-    "q38_kernel_timer",
+    "q38_kernel_timer", "q38_paged_append", "q38_paged_attention", "q38_paged_attention_scratch",
 )
 
 
@@ -91,9 +92,13 @@ def library() -> ctypes.CDLL:
     lib.q38_spec_step_graph.argtypes = [p] * 10
     lib.q38_verify_step.argtypes = [p] * 10
     lib.q38_step_status.argtypes = [p, ctypes.POINTER(i), i, p]
+    lib.q38_paged_append.argtypes = [p, p, p, p]
+    lib.q38_paged_attention.argtypes = [p, p, p, p, sz, p]
+    lib.q38_paged_attention_scratch.argtypes = [p, p, i]
+    sizes = ("q38_fp8_linear_scratch", "q38_fp4_linear_scratch", "q38_tiles_size", "q38_paged_attention_scratch")
     for name in EXPORTS:
         if name not in ("q38_last_error", "q38_destroy"):
-            getattr(lib, name).restype = ctypes.c_size_t if name in ("q38_fp8_linear_scratch", "q38_fp4_linear_scratch", "q38_tiles_size") else ctypes.c_int
+            getattr(lib, name).restype = ctypes.c_size_t if name in sizes else ctypes.c_int
     _lib = lib
     return lib
 
@@ -342,4 +347,172 @@ def mlp_up(x: torch.Tensor | None, rows: int, k: int, tiles: torch.Tensor, scale
         out = torch.empty(lib.q38_tiles_size(rows, inter), dtype=torch.uint8, device=scratch.device)
     xp = None if x is None else ptr(x.contiguous())
     check(lib.q38_mlp_up(xp, rows, k, ptr(tiles), ptr(scales), inter, ptr(scratch), ptr(out), stream()))
+    return out
+
+
+# ------------------------------------------------------------------------------------------------ the paged 8-bit cache
+
+
+class PagedCache(NamedTuple):
+    """One layer's keys and values in pages of 8-bit values (`q38_paged_cache`): k uint8 (e4m3) [pages, kv_heads, page, hd], v uint8
+    (e4m3) [pages, kv_heads, page / 16, hd, 16], k_scale, v_scale uint8 (E8M0) [pages, kv_heads]. `paged_cache` makes one."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+
+def paged_cache(pages: int, kv_heads: int, head_dim: int, page_size: int = 64, device="cuda") -> PagedCache:
+    """An empty cache: zeros, every page's scale 1."""
+    zeros = lambda *shape: torch.zeros(*shape, dtype=torch.uint8, device=device)  # noqa: E731
+    return PagedCache(zeros(pages, kv_heads, page_size, head_dim), zeros(pages, kv_heads, page_size // 16, head_dim, 16),
+                      zeros(pages, kv_heads) + 127, zeros(pages, kv_heads) + 127)
+
+
+def paged_values(cache: PagedCache) -> tuple[torch.Tensor, torch.Tensor]:
+    """What a cache holds as float32: keys and values [pages, kv_heads, page, hd]."""
+    times = lambda b: torch.ldexp(torch.ones((), device=b.device), b.int() - 127)[:, :, None, None]  # noqa: E731
+    e4m3 = lambda x: x.view(torch.float8_e4m3fn).float()  # noqa: E731
+    return e4m3(cache.k) * times(cache.k_scale), e4m3(cache.v).transpose(-1, -2).flatten(2, 3) * times(cache.v_scale)
+
+
+class _CacheArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + [
+        (n, ctypes.c_int) for n in ("pages", "kv_heads", "head_dim", "page_size")]
+
+
+class _RowArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("position", "pages", "q_start")] + [
+        (n, ctypes.c_int) for n in ("rows", "max_pages", "tokens", "max_tokens")]
+
+
+class _TokenArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("k", "v", "q", "q_out")]
+                + [(n, ctypes.c_longlong) for n in ("k_token", "k_head", "v_token", "v_head", "q_token", "q_head")]
+                + [("q_heads", ctypes.c_int), ("rotary_dim", ctypes.c_int)]
+                + [(n, ctypes.c_void_p) for n in ("cos", "sin", "q_norm", "k_norm")] + [("eps", ctypes.c_float)])
+
+
+class _QueryArgs(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("out", ctypes.c_void_p), ("q_heads", ctypes.c_int), ("scale", ctypes.c_float),
+                ("cap", ctypes.c_float), ("window", ctypes.c_int), ("slopes", ctypes.c_void_p), ("prefix", ctypes.c_void_p)]
+
+
+def _want(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, device: torch.device) -> int:
+    """The device pointer of a contiguous tensor of this type, shape and device; ValueError if it is another."""
+    if t.dtype is not dtype or t.shape != shape or t.device != device:
+        raise ValueError(f"{name} must be {dtype} {list(shape)} on {device}, got {t.dtype} {list(t.shape)} on {t.device}")
+    return ptr(t)
+
+
+def _heads_of(name: str, t: torch.Tensor, tokens: int | None, head_dim: int, device: torch.device) -> tuple[int, int, int]:
+    """Pointer and token and head strides of bf16 [tokens, heads, head_dim] whose last dim is contiguous."""
+    if t.dtype is not torch.bfloat16 or t.dim() != 3 or t.shape[2] != head_dim or t.device != device or (tokens is not None and t.shape[0] != tokens):
+        raise ValueError(f"{name} must be torch.bfloat16 [{'tokens' if tokens is None else tokens}, heads, {head_dim}] on {device}, got {t.dtype} {list(t.shape)} on {t.device}")
+    token, head, one = t.stride()
+    if one != 1:
+        raise ValueError(f"{name}'s last dim must be contiguous")
+    return t.data_ptr(), token, head
+
+
+def _paged_args(cache: PagedCache, position: torch.Tensor, pages: torch.Tensor, tokens: int, q_start, max_tokens):
+    """The cache and the rows of a call as the library takes them."""
+    k, device = cache.k, cache.k.device
+    if not k.is_cuda or k.dim() != 4:
+        raise ValueError("the cache must be on a device, its keys [pages, kv_heads, page, head_dim]")
+    count, heads, size, hd = k.shape
+    u8 = torch.uint8
+    c = _CacheArgs(_want("cache.k", k, u8, (count, heads, size, hd), device), _want("cache.v", cache.v, u8, (count, heads, size // 16, hd, 16), device),
+                   _want("cache.k_scale", cache.k_scale, u8, (count, heads), device),
+                   _want("cache.v_scale", cache.v_scale, u8, (count, heads), device), count, heads, hd, size)
+    if pages.dim() != 2:
+        raise ValueError(f"pages must be [rows, max_pages], got {list(pages.shape)}")
+    rows, width = pages.shape
+    if q_start is None:
+        if rows < 1 or tokens % rows:
+            raise ValueError(f"{tokens} tokens are not the same number in each of {rows} rows: say where they start (q_start)")
+        max_tokens = tokens // rows
+    elif max_tokens is None:
+        raise ValueError("ragged rows (q_start) need max_tokens, the most tokens of a row")
+    i32 = torch.int32
+    r = _RowArgs(_want("position", position, i32, (rows,), device), _want("pages", pages, i32, (rows, width), device),
+                 None if q_start is None else _want("q_start", q_start, i32, (rows + 1,), device), rows, width, tokens, min(max_tokens, tokens))
+    return c, r, device
+
+
+def _paged_call(device: torch.device, call) -> None:
+    """call(stream) on the device's current stream."""
+    if device.index == torch.cuda.current_device():
+        check(call(stream()))
+    else:
+        with torch.cuda.device(device):
+            check(call(stream()))
+
+
+def paged_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, position: torch.Tensor, pages: torch.Tensor, *, cos=None, sin=None,
+                 q=None, q_start=None, max_tokens: int | None = None, q_norm=None, k_norm=None, eps: float = 1e-6, q_out=None):
+    """Append bf16 keys and values [tokens, kv_heads, hd] to the rows' pages (`q38_paged_append`): normed (k_norm) and rotated (cos,
+    sin bf16 [tokens, rotary_dim]) on the way, coded to e4m3 with a power of two per page and head. position int32 [rows] is each
+    row's first new position (negative: the row is skipped), pages int32 [rows, max_pages] its page table, q_start int32 [rows + 1]
+    where its tokens start (None: the same number in each row; else max_tokens is the most that a row has). With queries q
+    [tokens, q_heads, hd] they are normed and rotated beside the keys and returned (in q_out, or a new tensor)."""
+    tokens = k.shape[0]
+    c, r, device = _paged_args(cache, position, pages, tokens, q_start, max_tokens)
+    t = _TokenArgs()
+    t.k, t.k_token, t.k_head = _heads_of("k", k, None, c.head_dim, device)
+    t.v, t.v_token, t.v_head = _heads_of("v", v, tokens, c.head_dim, device)
+    if k.shape[1] != c.kv_heads or v.shape[1] != c.kv_heads:
+        raise ValueError(f"keys and values of {c.kv_heads} heads, got {k.shape[1]} and {v.shape[1]}")
+    bf = torch.bfloat16
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin go together")
+    if cos is not None:
+        if cos.dim() != 2:
+            raise ValueError(f"cos must be [tokens, rotary_dim], got {list(cos.shape)}")
+        t.rotary_dim = cos.shape[1]
+        t.cos, t.sin = _want("cos", cos, bf, (tokens, t.rotary_dim), device), _want("sin", sin, bf, (tokens, t.rotary_dim), device)
+    if k_norm is not None:
+        t.k_norm = _want("k_norm", k_norm, bf, (c.head_dim,), device)
+    if q is not None:
+        t.q, t.q_token, t.q_head = _heads_of("q", q, tokens, c.head_dim, device)
+        t.q_heads = q.shape[1]
+        if q_norm is not None:
+            t.q_norm = _want("q_norm", q_norm, bf, (c.head_dim,), device)
+        if q_out is None:
+            q_out = torch.empty(tokens, t.q_heads, c.head_dim, dtype=bf, device=device)
+        t.q_out = _want("q_out", q_out, bf, (tokens, t.q_heads, c.head_dim), device)
+    elif q_norm is not None or q_out is not None:
+        raise ValueError("q_norm and q_out need q")
+    t.eps = eps
+    ref = ctypes.byref
+    _paged_call(device, lambda s: library().q38_paged_append(ref(c), ref(r), ref(t), s))
+    return q_out
+
+
+def paged_attention(cache: PagedCache, q: torch.Tensor, position: torch.Tensor, pages: torch.Tensor, *, q_start=None, max_tokens: int | None = None,
+                    scale: float | None = None, cap: float = 0.0, slopes=None, window: int = 0, prefix=None, out=None, scratch=None):
+    """Attention of bf16 queries [tokens, q_heads, hd] over their rows' pages, the queries' own positions among them (appended
+    before; rows as `paged_append` takes them): `q38_paged_attention`. scale None is hd ** -0.5; cap > 0 caps the scores by
+    cap * tanh(score / cap); slopes float32 [q_heads] add slope * (j - i); window > 0 sees the last `window` positions; prefix int32
+    [rows]: positions below it are seen by every token. Returns bf16 [tokens, q_heads, hd] (in out, or a new tensor)."""
+    if q.dim() != 3:
+        raise ValueError(f"q must be [tokens, q_heads, hd], got {list(q.shape)}")
+    tokens, heads, hd = q.shape
+    c, r, device = _paged_args(cache, position, pages, tokens, q_start, max_tokens)
+    shape = (tokens, heads, c.head_dim)
+    qp = _want("q", q, torch.bfloat16, shape, device)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.bfloat16, device=device)
+    a = _QueryArgs(qp, _want("out", out, torch.bfloat16, shape, device), heads, hd**-0.5 if scale is None else scale, cap, window)
+    if slopes is not None:
+        a.slopes = _want("slopes", slopes, torch.float32, (heads,), device)
+    if prefix is not None:
+        a.prefix = _want("prefix", prefix, torch.int32, (r.rows,), device)
+    ref, lib = ctypes.byref, library()
+    need = lib.q38_paged_attention_scratch(ref(c), ref(r), heads)
+    if scratch is None and need:
+        scratch = torch.empty(need, dtype=torch.uint8, device=device)
+    size = 0 if scratch is None else scratch.numel() * scratch.element_size()
+    _paged_call(device, lambda s: lib.q38_paged_attention(ref(c), ref(r), ref(a), ptr(scratch), size, s))
     return out
