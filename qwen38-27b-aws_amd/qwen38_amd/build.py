@@ -29,7 +29,7 @@ FLAGS = [
     "-Wno-unused-function",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
-SOURCES = ["gemm.hip", "fp4.hip", "norm.hip", "gdn.hip", "attn.hip", "prefill.hip", "paged.hip", "pick.hip", "pack.hip", "spec.hip",
+SOURCES = ["gemm.hip", "fp4.hip", "norm.hip", "gdn.hip", "attn.hip", "prefill.hip", "paged.hip", "paged_attn.hip", "pick.hip", "pack.hip", "spec.hip",
            "noalloc.hip", "engine.cpp"]
 
 

@@ -20,6 +20,15 @@ struct PagedAppendArgs {
     int visits, kv_blocks;   // set by the launcher: pages that a row may touch; workgroups of keys and values
 };
 
+// How a call of the attention is cut: from the host's sizes and the device's CUs, the same for the scratch's size and the launch.
+struct PagedPlan {
+    int few;                 // rows with at most this many (token, query head) pairs per KV head stream their positions, 16 pairs a tile
+    int target;              // workgroups that their positions are cut into, about
+    int items, slots;        // workgroups of those at most, and of them those that leave partial sums
+    size_t table, part, bytes;  // places in the scratch: the (row, KV head)s' first slot and count, the partial sums; its size
+};
+PagedPlan paged_attention_plan(const PagedCache& c, const PagedRows& r, int q_heads);
+
 struct PagedAttnArgs {
     PagedCache c;
     PagedRows r;
@@ -30,7 +39,44 @@ struct PagedAttnArgs {
     int window;
     const float* slopes;     // [q_heads] or null
     const int* prefix;       // [rows] or null
+    PagedPlan plan;
+    uint8_t* scratch;
 };
+
+constexpr float QNAN = __builtin_nanf("");
+
+// A row's new tokens: [t0, t0 + n) of the call's, at positions p0 .. p0 + n - 1 (p0 at most the table's end, past which no
+// page is found). A row to be skipped has n = 0.
+struct PagedRow {
+    int t0, n, p0;
+    bool skip;
+};
+
+__device__ __forceinline__ PagedRow paged_row(const PagedRows& a, int row, int page_size) {
+    PagedRow r;
+    int t1;
+    if (a.q_start) {
+        r.t0 = a.q_start[row];
+        t1 = a.q_start[row + 1];
+    } else {
+        r.t0 = row * a.max_tokens;
+        t1 = r.t0 + a.max_tokens;
+    }
+    r.t0 = min(max(r.t0, 0), a.tokens);
+    t1 = min(max(t1, r.t0), a.tokens);
+    const int p = a.position[row];
+    r.skip = p < 0;
+    r.n = min(t1 - r.t0, a.max_tokens);
+    r.p0 = min(p, a.max_pages * page_size);
+    return r;
+}
+
+// The page that holds position p of the row whose table entries are at `table`, or -1.
+__device__ __forceinline__ int paged_find(const PagedRows& a, const int* table, int page, int pages) {
+    if (page < 0 || page >= a.max_pages) return -1;
+    const int id = table[page];
+    return id >= 0 && id < pages ? id : -1;
+}
 
 hipError_t q38_paged_append(const PagedAppendArgs& a, hipStream_t stream);
 hipError_t q38_paged_attention(const PagedAttnArgs& a, hipStream_t stream);

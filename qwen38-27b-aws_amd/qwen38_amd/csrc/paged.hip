@@ -12,41 +12,6 @@
 
 namespace {
 
-constexpr float QNAN = __builtin_nanf("");
-
-// A row's new tokens: [t0, t0 + n) of the call's, at positions p0 .. p0 + n - 1 (p0 at most the table's end, past which no
-// page is found). A row to be skipped has n = 0.
-struct PagedRow {
-    int t0, n, p0;
-    bool skip;
-};
-
-__device__ __forceinline__ PagedRow paged_row(const PagedRows& a, int row, int page_size) {
-    PagedRow r;
-    int t1;
-    if (a.q_start) {
-        r.t0 = a.q_start[row];
-        t1 = a.q_start[row + 1];
-    } else {
-        r.t0 = row * a.max_tokens;
-        t1 = r.t0 + a.max_tokens;
-    }
-    r.t0 = min(max(r.t0, 0), a.tokens);
-    t1 = min(max(t1, r.t0), a.tokens);
-    const int p = a.position[row];
-    r.skip = p < 0;
-    r.n = min(t1 - r.t0, a.max_tokens);
-    r.p0 = min(p, a.max_pages * page_size);
-    return r;
-}
-
-// The page that holds position p of the row whose table entries are at `table`, or -1.
-__device__ __forceinline__ int paged_find(const PagedRows& a, const int* table, int page, int pages) {
-    if (page < 0 || page >= a.max_pages) return -1;
-    const int id = table[page];
-    return id >= 0 && id < pages ? id : -1;
-}
-
 // The scale byte that values up to amax need: 448 = 1.75 x 2^8.
 __device__ __forceinline__ int paged_need(float amax) {
     const uint32_t bits = __float_as_uint(amax);
@@ -288,89 +253,6 @@ hipError_t q38_paged_append(const PagedAppendArgs& a0, hipStream_t stream) {
     return hipGetLastError();
 }
 
-// A wave per token and query head: its lanes take 64 positions' scores, then, position by position, E dims each.
-template <int E>
-__global__ __launch_bounds__(64) void paged_attention_kernel(const PagedAttnArgs a) {
-    constexpr int HD = E * 64;
-    __shared__ float q[HD];
-    const int lane = threadIdx.x, hq = blockIdx.x % a.q_heads, i = blockIdx.x / a.q_heads % a.r.max_tokens, row = blockIdx.x / a.q_heads / a.r.max_tokens;
-    const int G = a.q_heads / a.c.kv_heads, kvh = hq / G, ps = a.c.page_size;
-    const PagedRow r = paged_row(a.r, row, ps);
-    if (i >= r.n) return;
-    const size_t at = ((size_t)(r.t0 + i) * a.q_heads + hq) * HD + lane * E;
-    float o[E] = {}, x[E];
-    float m = -INFINITY, l = 0.0f;
-    if (!r.skip) {
-        load_dims<E>(a.q + at, x);
-#pragma unroll
-        for (int e = 0; e < E; ++e) q[lane * E + e] = x[e];
-        __syncthreads();
-        const int p = r.p0 + i, total = r.p0 + r.n;
-        const int hi = min(total, max(p + 1, a.prefix ? a.prefix[row] : 0)), lo = a.window ? max(0, p + 1 - a.window) : 0;
-        const float slope = a.slopes ? a.slopes[hq] : 0.0f;
-        const int* table = a.r.pages + (size_t)row * a.r.max_pages;
-        for (int base = lo / 64 * 64; base < hi; base += 64) {
-            const int j = base + lane, id = paged_find(a.r, table, j / ps, a.c.pages);
-            float s = -INFINITY;
-            if (j >= lo && j < hi) {
-                s = QNAN;
-                if (id >= 0) {
-                    const size_t head = (size_t)id * a.c.kv_heads + kvh;
-                    const uint32_t* kp = (const uint32_t*)(a.c.k + (head * ps + j % ps) * HD);
-                    s = 0.0f;
-                    for (int d = 0; d < HD / 4; ++d) {
-                        typedef float v2f_ __attribute__((ext_vector_type(2)));
-                        const uint32_t w = kp[d];
-                        const v2f_ f0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, 1.0f, false), f1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, 1.0f, true);
-                        s += q[d * 4] * f0[0] + q[d * 4 + 1] * f0[1] + q[d * 4 + 2] * f1[0] + q[d * 4 + 3] * f1[1];
-                    }
-                    s *= ldexpf(a.scale, a.c.k_scale[head] - 127);
-                    if (a.cap > 0.0f) s = a.cap * tanhf(s / a.cap);
-                    s += slope * (float)(j - p);
-                }
-            }
-            const float mn = fmaxf(m, warp_max(s)), safe = mn == -INFINITY ? 0.0f : mn, f = expf(m - safe), w = expf(s - safe);
-            m = mn;
-            l = l * f + warp_sum(w);
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[e] *= f;
-            for (int y = 0; y < 64; ++y) {
-                const int jy = base + y;
-                if (jy < lo || jy >= hi) continue;
-                const int idy = __shfl(id, y);
-                const float wy = __shfl(w, y);
-                if (idy < 0) continue;
-                const size_t head = (size_t)idy * a.c.kv_heads + kvh;
-                const float sc = ldexpf(wy, a.c.v_scale[head] - 127);
-                const uint8_t* vp = a.c.v + head * ps * HD + ((size_t)(jy % ps / 16) * HD + lane * E) * 16 + jy % 16;
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    typedef float v2f_ __attribute__((ext_vector_type(2)));
-                    const v2f_ f0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8((uint32_t)vp[e * 16], 1.0f, false);
-                    o[e] += sc * f0[0];
-                }
-            }
-        }
-    }
-    const float inv = m == -INFINITY && l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-    for (int e = 0; e < E; ++e) a.out[at + e] = f2bf(o[e] * inv);
-}
-
-hipError_t q38_paged_attention(const PagedAttnArgs& a, hipStream_t stream) {
-    const size_t grid = (size_t)a.r.rows * a.r.max_tokens * a.q_heads;
-    if (!grid) return hipSuccess;
-#define ATTEND(E) hipLaunchKernelGGL((paged_attention_kernel<E>), dim3(grid), dim3(64), 0, stream, a)
-    switch (a.c.head_dim) {
-        case 64: ATTEND(1); break;
-        case 128: ATTEND(2); break;
-        case 256: ATTEND(4); break;
-        default: return hipErrorInvalidValue;
-    }
-#undef ATTEND
-    return hipGetLastError();
-}
-
 // ---- The C ABI (include/q38.h).
 namespace {
 
@@ -431,7 +313,10 @@ int q38_paged_append(const q38_paged_cache* c, const q38_paged_rows* r, const q3
     return e == hipSuccess ? 0 : q38_report(hipGetErrorString(e));
 }
 
-size_t q38_paged_attention_scratch(const q38_paged_cache* c, const q38_paged_rows* r, int q_heads) { return 0; }
+size_t q38_paged_attention_scratch(const q38_paged_cache* c, const q38_paged_rows* r, int q_heads) {
+    if (paged_bad(c, r) || q_heads < 1 || q_heads % c->kv_heads || q_heads / c->kv_heads > 64) return 0;
+    return paged_attention_plan(*c, *r, q_heads).bytes;
+}
 
 int q38_paged_attention(const q38_paged_cache* c, const q38_paged_rows* r, const q38_paged_query* q, void* scratch, size_t scratch_bytes,
                         void* stream) {
@@ -455,6 +340,10 @@ int q38_paged_attention(const q38_paged_cache* c, const q38_paged_rows* r, const
     a.window = q->window;
     a.slopes = q->slopes;
     a.prefix = q->prefix;
+    a.plan = paged_attention_plan(*c, *r, q->q_heads);
+    if (a.plan.bytes > scratch_bytes || (a.plan.bytes && !scratch)) return q38_report("paged attention: the scratch is smaller than q38_paged_attention_scratch says");
+    if ((uintptr_t)scratch % 256) return q38_report("paged attention: the scratch must be 256-byte aligned");
+    a.scratch = (uint8_t*)scratch;
     const hipError_t e = q38_paged_attention(a, (hipStream_t)stream);
     return e == hipSuccess ? 0 : q38_report(hipGetErrorString(e));
 }

@@ -1,0 +1,506 @@
+// Attention over the paged 8-bit cache (paged.hip, include/q38.h): o_i = sum_j softmax_j(score_ij) v_j over the positions j that
+// token i sees.
+//
+// Keys and values are widened to bf16 in registers, exactly (an e4m3 value times a power of two), for the bf16 matrix cores;
+// scores, their maxima and the sums stay in float32, the weights are rounded to bf16 for the second product (2^-8 of each, as
+// the output's own rounding) and summed unrounded. Exponentials are powers of two: scores carry log2 e.
+//
+// The maximum that the weights are relative to is raised, and the sums so far rescaled, only when a score passes it by
+// SLACK: until then weights reach 2^SLACK, which float32 and bf16 hold as exactly as those below one.
+#include <algorithm>
+
+#include "kernels.h"
+#include "paged.h"
+
+namespace {
+
+constexpr float LOG2E = 1.44269504088896340736f, SLACK = 8.0f;
+
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// What a packed query row (token r / G, query head r % G of the KV head's G) sees: positions [lo, hi); at is its own.
+struct PagedSight {
+    int lo, hi, at;
+};
+
+__device__ __forceinline__ PagedSight paged_sight(const PagedAttnArgs& a, const PagedRow& r, int prefix, int i) {
+    const int at = r.p0 + i;
+    return {a.window ? max(0, at + 1 - a.window) : 0, min(r.p0 + r.n, max(at + 1, prefix)), at};
+}
+
+// Eight e4m3 codes times a power of two as one bf16 matrix operand.
+__device__ __forceinline__ v8bf16 paged_widen(uint32_t w0, uint32_t w1, float scale) {
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    const u4 r = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, scale, false)),
+                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, scale, true)),
+                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale, false)),
+                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale, true))};
+    return __builtin_bit_cast(v8bf16, r);
+}
+
+__device__ __forceinline__ float paged_scale(int byte) { return __uint_as_float((uint32_t)byte << 23); }
+
+// Scores to powers of two: capped and biased as the call asks.
+template <int N>
+__device__ __forceinline__ void paged_scores(const PagedAttnArgs& a, float (&s)[N], float slope2, int j0, int at) {
+    if (a.cap > 0.0f) {
+        const float in = a.scale * 2.0f * LOG2E / a.cap, out = a.cap * LOG2E;  // tanh x = 1 - 2 / (e^2x + 1)
+#pragma unroll
+        for (int e = 0; e < N; ++e) s[e] = out - 2.0f * out * __builtin_amdgcn_rcpf(exp2_(s[e] * in) + 1.0f);
+    } else {
+        const float f = a.scale * LOG2E;
+#pragma unroll
+        for (int e = 0; e < N; ++e) s[e] *= f;
+    }
+    if (a.slopes) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) s[e] += slope2 * (float)(j0 + e - at);
+    }
+}
+
+}  // namespace
+
+// ---- Few query rows (decode, verify): the positions streamed once from memory, straight into registers.
+//
+// A wave takes 64 positions of one (row, KV head) at a time, its four lane groups g of 16 lanes 16 positions each, with all of the
+// row's query rows as columns (16 per tile of the matrix cores, NT tiles). Keys are A (a 16-position block's rows permuted, so
+// that a lane's 16 scores of the four blocks are its group's 16 positions in order: they are the second product's B operand
+// as they stand, without moving between lanes); values are A of the second product, sixteen positions of a dim being one 16-byte load.
+// Nothing goes through LDS until a workgroup's four waves, which take tiles in turn, put their sums together.
+//
+// Bound: the cache's bytes from memory. With one tile of query rows two waves per SIMD keep 64 KB of loads in flight per
+// SIMD's pair; with more, the sums and the queries take a wave's whole register file, and one wave per SIMD.
+//
+// The work is cut on the device, where the lengths are: units of 256 positions (a tile for each wave) of every row and KV head, as many per workgroup
+// as give PAGED_PER_CU workgroups per CU, rows in order. A (row, KV head) that one workgroup has all of is written out by it; the others'
+// sums go to scratch slots, which paged_join_kernel puts together.
+namespace {
+
+constexpr int PAGED_PER_CU = 4;  // workgroups that the work is cut into, per CU
+
+struct PagedItem {
+    int row, kvh, chunk, chunks, slot;  // slot: the item's place among the partial sums, -1 if it has its (row, KV head) whole
+};
+
+// Units of a row that streams; 0 for one that does not.
+__device__ __forceinline__ int paged_units(const PagedAttnArgs& a, int row, int G) {
+    const PagedRow r = paged_row(a.r, row, a.c.page_size);
+    if (r.n <= 0 || r.n * G > a.plan.few) return 0;
+    if (r.skip) return 1;
+    const int lo = a.window ? max(0, r.p0 + 1 - a.window) / 64 : 0;
+    return max(1, ((r.p0 + r.n + 63) / 64 - lo + 3) / 4);
+}
+
+__device__ __forceinline__ bool paged_item(const PagedAttnArgs& a, int id, int G, int target, PagedItem& it) {
+    const int lane = threadIdx.x & 63, Hkv = a.c.kv_heads;
+    double total = 0.0;
+    for (int row = lane; row < a.r.rows; row += 64) total += paged_units(a, row, G);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
+    const int per = max(1, (int)((total * Hkv + (target - 1)) / target));
+    int before = 0, slots = 0;  // items and slots of the rows so far
+    for (int base = 0; base < a.r.rows; base += 64) {
+        const int row = base + lane;
+        const int n = row < a.r.rows ? (paged_units(a, row, G) + per - 1) / per : 0, m = n > 1 ? n : 0;
+        int ends = n, slot_ends = m;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int x = __shfl_up(ends, o), y = __shfl_up(slot_ends, o);
+            if (lane >= o) ends += x, slot_ends += y;
+        }
+        const unsigned long long past = __ballot(before + ends * Hkv > id);
+        if (past) {
+            const int l = __ffsll(past) - 1;
+            const int chunks = __shfl(n, l), first = before + (__shfl(ends, l) - chunks) * Hkv, slot0 = slots + (__shfl(slot_ends, l) - (chunks > 1 ? chunks : 0)) * Hkv;
+            it.row = base + l;
+            it.chunks = chunks;
+            it.kvh = (id - first) / chunks;
+            it.chunk = (id - first) % chunks;
+            it.slot = chunks > 1 ? slot0 + id - first : -1;
+            return true;
+        }
+        before += __shfl(ends, 63) * Hkv;
+        slots += __shfl(slot_ends, 63) * Hkv;
+    }
+    return false;
+}
+
+}  // namespace
+
+template <int HD, int NT>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT > 1 ? 1 : 2, NT > 1 ? 1 : 2))) void paged_stream_kernel(const PagedAttnArgs a) {
+    constexpr int KB = HD / 64, DB = HD / 16, LD = HD + 4;
+    __shared__ __attribute__((aligned(16))) float sums[4 * 16 * LD];
+    __shared__ float tops[4][16 * NT], totals[4][16 * NT];
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+    const int Hkv = a.c.kv_heads, G = a.q_heads / Hkv, ps = a.c.page_size, shift = __builtin_ctz(ps);
+    PagedItem it;
+    if (!paged_item(a, blockIdx.x, G, a.plan.target, it)) return;
+    it.row = __builtin_amdgcn_readfirstlane(it.row);
+    it.kvh = __builtin_amdgcn_readfirstlane(it.kvh);
+    const PagedRow r = paged_row(a.r, it.row, ps);
+    const int R = r.n * G, total = r.p0 + r.n;
+    if (it.chunk == 0 && threadIdx.x == 0) {
+        int2* t = (int2*)(a.scratch + a.plan.table);
+        t[it.row * Hkv + it.kvh] = make_int2(it.slot, it.chunks);
+    }
+    const int prefix = a.prefix ? a.prefix[it.row] : 0;
+    const int lo_all = a.window ? max(0, r.p0 + 1 - a.window) : 0, t_first = lo_all / 64, t_count = r.skip ? 0 : (total + 63) / 64 - t_first;
+    const int t0 = t_first + (int)((long long)t_count * it.chunk / it.chunks), t1 = t_first + (int)((long long)t_count * (it.chunk + 1) / it.chunks);
+    const int lo_last = a.window ? max(0, total - a.window) : 0, hi_first = min(total, max(r.p0 + 1, prefix));  // what every token sees
+    const int* table = a.r.pages + (size_t)it.row * a.r.max_pages;
+
+    v8bf16 qf[NT][KB][2];
+    PagedSight see[NT];
+    float slope2[NT], top[NT], sum[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int row = nt * 16 + col, i = row / G, head = it.kvh * G + row % G;
+        const bool live = row < R;
+        see[nt] = live ? paged_sight(a, r, prefix, i) : PagedSight{0, 0, 0};
+        slope2[nt] = live && a.slopes ? a.slopes[head] * LOG2E : 0.0f;
+        top[nt] = -INFINITY;
+        sum[nt] = 0.0f;
+        const bf16_t* qp = a.q + ((size_t)(r.t0 + (live ? i : 0)) * a.q_heads + (live ? head : 0)) * HD + g * 16;
+#pragma unroll
+        for (int j = 0; j < KB; ++j)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                qf[nt][j][u] = *(const v8bf16*)(qp + j * 64 + u * 8);
+                if (!live) qf[nt][j][u] = (v8bf16)(__bf16)0.0f;
+            }
+    }
+    v4f o[NT][DB];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[nt][d] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+
+    // The pages of a tile's key rows (lane group col / 4 of each block) and of its values (lane group g); -1: none.
+    auto find = [&](int t, int group) { return paged_find(a.r, table, (t * 64 + group * 16) >> shift, a.c.pages); };
+    uint4 kr[4][KB], vr[DB];
+    float ks, vs;
+    auto load_keys = [&](int t, int id) __attribute__((always_inline)) {
+        const size_t head = (size_t)max(id, 0) * Hkv + it.kvh;
+        const int slot = (t * 64 + (col >> 2) * 16 + (col & 3)) & (ps - 1);
+        const uint8_t* p = a.c.k + (head * ps + slot) * HD + g * 16;
+        ks = paged_scale(a.c.k_scale[head]);
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int j = 0; j < KB; ++j) kr[b][j] = *(const uint4*)(p + b * 4 * HD + j * 64);
+    };
+    auto load_values = [&](int t, int id) __attribute__((always_inline)) {
+        const size_t head = (size_t)max(id, 0) * Hkv + it.kvh;
+        const uint8_t* p = a.c.v + head * ps * HD + ((size_t)(((t * 64 + g * 16) & (ps - 1)) >> 4) * HD + col) * 16;
+        vs = paged_scale(a.c.v_scale[head]);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) vr[d] = *(const uint4*)(p + d * 256);
+    };
+    int t = t0 + wv;
+    int idk = 0, idv = 0, next_k = 0, next_v = 0;
+    if (t < t1) {
+        idk = find(t, col >> 2);
+        idv = find(t, g);
+        if (t + 4 < t1) next_k = find(t + 4, col >> 2), next_v = find(t + 4, g);
+        load_keys(t, idk);
+        load_values(t, idv);
+    }
+    for (; t < t1; t += 4) {
+        float s[NT][16];
+        {
+            v4f c[NT][4];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+#pragma unroll
+                for (int j = 0; j < KB; ++j)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const v8bf16 kf = u ? paged_widen(kr[b][j].z, kr[b][j].w, ks) : paged_widen(kr[b][j].x, kr[b][j].y, ks);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+                            c[nt][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[nt][j][u], j + u ? c[nt][b] : (v4f){0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+                    }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[nt][e] = c[nt][e >> 2][e & 3];
+        }
+        const bool more = t + 4 < t1;
+        int after_k = 0, after_v = 0;
+        if (more) {
+            if (t + 8 < t1) after_k = find(t + 8, col >> 2), after_v = find(t + 8, g);
+            load_keys(t + 4, next_k);
+        }
+        const int base = t * 64, mine = base + g * 16;
+        const bool edge = base < lo_last || base + 64 > hi_first || __any(idv < 0);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            paged_scores<16>(a, s[nt], slope2[nt], mine, see[nt].at);
+            if (edge)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[nt][e] = mine + e < see[nt].lo || mine + e >= see[nt].hi ? -INFINITY : idv < 0 ? QNAN : s[nt][e];
+            float m = s[nt][0];
+#pragma unroll
+            for (int e = 1; e < 16; ++e) m = fmaxf(m, s[nt][e]);
+            m = fmaxf(m, __shfl_xor(m, 16));
+            m = fmaxf(m, __shfl_xor(m, 32));
+            if (__any(m > top[nt] + SLACK || (top[nt] == -INFINITY && m > -INFINITY))) {
+                const float up = fmaxf(top[nt], m), f = up == -INFINITY ? 1.0f : exp2_(top[nt] - up);
+                top[nt] = up;
+                sum[nt] *= f;
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[nt][d][e] *= f;
+            }
+            const float from = top[nt] == -INFINITY ? 0.0f : top[nt];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                s[nt][e] = exp2_(s[nt][e] - from);
+                sum[nt] += s[nt][e];
+            }
+        }
+        if (base + 64 > total || __any(idv < 0)) {  // bytes that no token wrote may be anything
+            const int live = idv < 0 ? 0 : total - mine;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                uint32_t* w = (uint32_t*)&vr[d];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) w[x] &= live >= 4 * x + 4 ? 0xffffffffu : live <= 4 * x ? 0u : (1u << 8 * (live - 4 * x)) - 1;
+            }
+        }
+        v8bf16 pf[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+                const u4 w = {pk_bf16(s[nt][8 * u], s[nt][8 * u + 1]), pk_bf16(s[nt][8 * u + 2], s[nt][8 * u + 3]),
+                              pk_bf16(s[nt][8 * u + 4], s[nt][8 * u + 5]), pk_bf16(s[nt][8 * u + 6], s[nt][8 * u + 7])};
+                pf[nt][u] = __builtin_bit_cast(v8bf16, w);
+            }
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const v8bf16 vf = u ? paged_widen(vr[d].z, vr[d].w, vs) : paged_widen(vr[d].x, vr[d].y, vs);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) o[nt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[nt][u], o[nt][d], 0, 0, 0);
+            }
+        if (more) load_values(t + 4, next_v);
+        idk = next_k;
+        idv = next_v;
+        next_k = after_k;
+        next_v = after_v;
+    }
+
+    // The waves' sums together.
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        sum[nt] += __shfl_xor(sum[nt], 16);
+        sum[nt] += __shfl_xor(sum[nt], 32);
+        if (g == 0) tops[wv][nt * 16 + col] = top[nt], totals[wv][nt * 16 + col] = sum[nt];
+    }
+    __syncthreads();
+    float* part = (float*)(a.scratch + a.plan.part) + (size_t)max(it.slot, 0) * a.plan.few * (HD + 2);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        if (nt * 16 >= R) break;
+        const int mine = nt * 16 + col;
+        const float up = fmaxf(fmaxf(tops[0][mine], tops[1][mine]), fmaxf(tops[2][mine], tops[3][mine]));
+        const float f = up == -INFINITY ? 1.0f : exp2_(top[nt] - up);
+        if (nt) __syncthreads();
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+            *(v4f*)(sums + (wv * 16 + col) * LD + d * 16 + g * 4) = (v4f){o[nt][d][0] * f, o[nt][d][1] * f, o[nt][d][2] * f, o[nt][d][3] * f};
+        __syncthreads();
+        for (int x = threadIdx.x; x < 16 * HD / 4; x += 256) {
+            const int c = x / (HD / 4), d = x % (HD / 4) * 4, row = nt * 16 + c;
+            if (row >= R) continue;
+            v4f v = *(const v4f*)(sums + c * LD + d);
+#pragma unroll
+            for (int w = 1; w < 4; ++w) v += *(const v4f*)(sums + (w * 16 + c) * LD + d);
+            const float m = fmaxf(fmaxf(tops[0][row], tops[1][row]), fmaxf(tops[2][row], tops[3][row]));
+            float l = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) l += totals[w][row] * (m == -INFINITY ? 1.0f : exp2_(tops[w][row] - m));
+            if (it.slot < 0) {
+                const float inv = r.skip ? 0.0f : 1.0f / l;
+                *(uint2*)(a.out + ((size_t)(r.t0 + row / G) * a.q_heads + it.kvh * G + row % G) * HD + d) =
+                    make_uint2(pk_bf16(v[0] * inv, v[1] * inv), pk_bf16(v[2] * inv, v[3] * inv));
+            } else {
+                *(v4f*)(part + (size_t)row * HD + d) = v;
+                if (d == 0) *(float2*)(part + (size_t)a.plan.few * HD + row * 2) = make_float2(m, l);
+            }
+        }
+    }
+}
+
+// The parts of one (row, KV head)'s query row put together. Grid: rows x KV heads x query rows.
+template <int E>
+__global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) {
+    constexpr int HD = E * 64;
+    __shared__ float sums[4][HD], totals[4];
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, Hkv = a.c.kv_heads, G = a.q_heads / Hkv;
+    const int q = blockIdx.x % a.plan.few, kvh = blockIdx.x / a.plan.few % Hkv, row = blockIdx.x / a.plan.few / Hkv;
+    const PagedRow r = paged_row(a.r, row, a.c.page_size);
+    if (q >= r.n * G || r.n * G > a.plan.few) return;
+    const int2 t = ((const int2*)(a.scratch + a.plan.table))[row * Hkv + kvh];
+    if (t.y <= 1) return;
+    const size_t step = (size_t)a.plan.few * (HD + 2);
+    const float* part = (const float*)(a.scratch + a.plan.part) + (size_t)t.x * step;
+    const float* stats = part + (size_t)a.plan.few * HD + q * 2;
+    float top = -INFINITY;
+    for (int c = lane; c < t.y; c += 64) top = fmaxf(top, stats[c * step]);
+    top = warp_max(top);
+    float o[E] = {}, l = 0.0f;
+    for (int c = wv; c < t.y; c += 4) {
+        const float2 s = *(const float2*)(stats + c * step);
+        const float f = s.x == -INFINITY ? (s.y == 0.0f ? 0.0f : 1.0f) : exp2_(s.x - top);  // no weights, or only NaN ones
+        l += s.y * f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] += part[c * step + (size_t)q * HD + e * 64 + lane] * f;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) sums[wv][e * 64 + lane] = o[e];
+    if (lane == 0) totals[wv] = l;
+    __syncthreads();
+    const float all = (totals[0] + totals[1]) + (totals[2] + totals[3]);
+    bf16_t* out = a.out + ((size_t)(r.t0 + q / G) * a.q_heads + kvh * G + q % G) * HD;
+    for (int d = threadIdx.x; d < HD; d += 256) out[d] = f2bf(((sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d])) / all);
+}
+
+template <int E>
+__device__ __forceinline__ void load_dims(const bf16_t* p, float (&x)[E]) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = bf2f(p[e]);
+}
+
+// A wave per token and query head: its lanes take 64 positions' scores, then, position by position, E dims each.
+template <int E>
+__global__ __launch_bounds__(64) void paged_attention_kernel(const PagedAttnArgs a) {
+    constexpr int HD = E * 64;
+    __shared__ float q[HD];
+    const int lane = threadIdx.x, hq = blockIdx.x % a.q_heads, i = blockIdx.x / a.q_heads % a.r.max_tokens, row = blockIdx.x / a.q_heads / a.r.max_tokens;
+    const int G = a.q_heads / a.c.kv_heads, kvh = hq / G, ps = a.c.page_size;
+    const PagedRow r = paged_row(a.r, row, ps);
+    if (i >= r.n || (a.plan.items && r.n * G <= a.plan.few)) return;
+    const size_t at = ((size_t)(r.t0 + i) * a.q_heads + hq) * HD + lane * E;
+    float o[E] = {}, x[E];
+    float m = -INFINITY, l = 0.0f;
+    if (!r.skip) {
+        load_dims<E>(a.q + at, x);
+#pragma unroll
+        for (int e = 0; e < E; ++e) q[lane * E + e] = x[e];
+        __syncthreads();
+        const int p = r.p0 + i, total = r.p0 + r.n;
+        const int hi = min(total, max(p + 1, a.prefix ? a.prefix[row] : 0)), lo = a.window ? max(0, p + 1 - a.window) : 0;
+        const float slope = a.slopes ? a.slopes[hq] : 0.0f;
+        const int* table = a.r.pages + (size_t)row * a.r.max_pages;
+        for (int base = lo / 64 * 64; base < hi; base += 64) {
+            const int j = base + lane, id = paged_find(a.r, table, j / ps, a.c.pages);
+            float s = -INFINITY;
+            if (j >= lo && j < hi) {
+                s = QNAN;
+                if (id >= 0) {
+                    const size_t head = (size_t)id * a.c.kv_heads + kvh;
+                    const uint32_t* kp = (const uint32_t*)(a.c.k + (head * ps + j % ps) * HD);
+                    s = 0.0f;
+                    for (int d = 0; d < HD / 4; ++d) {
+                        typedef float v2f_ __attribute__((ext_vector_type(2)));
+                        const uint32_t w = kp[d];
+                        const v2f_ f0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, 1.0f, false), f1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, 1.0f, true);
+                        s += q[d * 4] * f0[0] + q[d * 4 + 1] * f0[1] + q[d * 4 + 2] * f1[0] + q[d * 4 + 3] * f1[1];
+                    }
+                    s *= ldexpf(a.scale, a.c.k_scale[head] - 127);
+                    if (a.cap > 0.0f) s = a.cap * tanhf(s / a.cap);
+                    s += slope * (float)(j - p);
+                }
+            }
+            const float mn = fmaxf(m, warp_max(s)), safe = mn == -INFINITY ? 0.0f : mn, f = expf(m - safe), w = expf(s - safe);
+            m = mn;
+            l = l * f + warp_sum(w);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] *= f;
+            for (int y = 0; y < 64; ++y) {
+                const int jy = base + y;
+                if (jy < lo || jy >= hi) continue;
+                const int idy = __shfl(id, y);
+                const float wy = __shfl(w, y);
+                if (idy < 0) continue;
+                const size_t head = (size_t)idy * a.c.kv_heads + kvh;
+                const float sc = ldexpf(wy, a.c.v_scale[head] - 127);
+                const uint8_t* vp = a.c.v + head * ps * HD + ((size_t)(jy % ps / 16) * HD + lane * E) * 16 + jy % 16;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    typedef float v2f_ __attribute__((ext_vector_type(2)));
+                    const v2f_ f0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8((uint32_t)vp[e * 16], 1.0f, false);
+                    o[e] += sc * f0[0];
+                }
+            }
+        }
+    }
+    const float inv = m == -INFINITY && l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int e = 0; e < E; ++e) a.out[at + e] = f2bf(o[e] * inv);
+}
+
+
+PagedPlan paged_attention_plan(const PagedCache& c, const PagedRows& r, int q_heads) {
+    PagedPlan p{};
+    const int G = q_heads / c.kv_heads;
+    const long long most = (long long)r.max_tokens * G;
+    // All rows stream while their query rows fit four tiles; in a ragged call with longer rows those of one tile of tokens.
+    p.few = (int)(most <= 64 ? (most + 15) / 16 * 16 : (G + 15) / 16 * 16);
+    const bool any = most <= 64 || r.q_start;
+    p.target = PAGED_PER_CU * q38_device_cus();
+    const long long heads = (long long)r.rows * c.kv_heads, units = ((long long)r.max_pages * c.page_size + r.max_tokens + 63) / 64 / 4 + 2;
+    p.items = any ? (int)std::min<long long>(p.target + heads, heads * units) : 0;
+    p.slots = units > 1 ? std::min(2 * p.target, p.items) : 0;
+    p.bytes = 0;
+    if (any) {
+        p.table = 0;
+        p.part = (size_t)heads * 8 + 255 & ~(size_t)255;
+        p.bytes = p.part + (size_t)p.slots * p.few * (c.head_dim + 2) * 4;
+    }
+    return p;
+}
+
+hipError_t q38_paged_attention(const PagedAttnArgs& a, hipStream_t stream) {
+    const int few = a.plan.few, G = a.q_heads / a.c.kv_heads;
+    if (a.plan.items) {
+#define STREAM(HD, NT) hipLaunchKernelGGL((paged_stream_kernel<HD, NT>), dim3(a.plan.items), dim3(256), 0, stream, a)
+#define STREAMS(HD)                  \
+    switch (few / 16) {              \
+        case 1: STREAM(HD, 1); break; \
+        case 2: STREAM(HD, 2); break; \
+        case 3: STREAM(HD, 3); break; \
+        case 4: STREAM(HD, 4); break; \
+        default: return hipErrorInvalidValue; \
+    }
+        switch (a.c.head_dim) {
+            case 64: STREAMS(64); break;
+            case 128: STREAMS(128); break;
+            case 256: STREAMS(256); break;
+            default: return hipErrorInvalidValue;
+        }
+        const size_t rows = (size_t)a.r.rows * a.c.kv_heads * few;
+        switch (a.plan.slots ? a.c.head_dim : 0) {
+            case 64: hipLaunchKernelGGL((paged_join_kernel<1>), dim3(rows), dim3(256), 0, stream, a); break;
+            case 128: hipLaunchKernelGGL((paged_join_kernel<2>), dim3(rows), dim3(256), 0, stream, a); break;
+            case 256: hipLaunchKernelGGL((paged_join_kernel<4>), dim3(rows), dim3(256), 0, stream, a); break;
+        }
+        if ((long long)a.r.max_tokens * G <= few) return hipGetLastError();
+    }
+    const size_t grid = (size_t)a.r.rows * a.r.max_tokens * a.q_heads;
+#define ATTEND(E) hipLaunchKernelGGL((paged_attention_kernel<E>), dim3(grid), dim3(64), 0, stream, a)
+    switch (a.c.head_dim) {
+        case 64: ATTEND(1); break;
+        case 128: ATTEND(2); break;
+        case 256: ATTEND(4); break;
+        default: return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
+}
