@@ -62,7 +62,7 @@ __device__ __forceinline__ void paged_scores(const PagedAttnArgs& a, float (&s)[
 
 // ---- Few query rows (decode, verify): the positions streamed once from memory, straight into registers.
 //
-// A wave takes 64 positions of one (row, KV head) at a time, its four lane groups g of 16 lanes 16 positions each, with all of the
+// A wave takes a tile of 4 PT positions of one (row, KV head) at a time, its four lane groups g of 16 lanes PT each, with all of the
 // row's query rows as columns (16 per tile of the matrix cores, NT tiles). Keys are A (a 16-position block's rows permuted, so
 // that a lane's 16 scores of the four blocks are its group's 16 positions in order: they are the second product's B operand
 // as they stand, without moving between lanes); values are A of the second product, sixteen positions of a dim being one 16-byte load.
@@ -127,9 +127,10 @@ __device__ __forceinline__ bool paged_item(const PagedAttnArgs& a, int id, int G
 
 }  // namespace
 
-template <int HD, int NT>
+template <int HD, int NT, int PT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT > 1 ? 1 : 2, NT > 1 ? 1 : 2))) void paged_stream_kernel(const PagedAttnArgs a) {
-    constexpr int KB = HD / 64, DB = HD / 16, LD = HD + 4;
+    constexpr int KB = HD / 64, DB = HD / 16, LD = HD + 4, NB = PT / 4, TILE = 4 * PT;
+    typedef uint32_t words __attribute__((ext_vector_type(PT / 4)));
     __shared__ __attribute__((aligned(16))) float sums[4 * 16 * LD];
     __shared__ float tops[4][16 * NT], totals[4][16 * NT];
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
@@ -145,12 +146,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT > 1 ? 1 
         t[it.row * Hkv + it.kvh] = make_int2(it.slot, it.chunks);
     }
     const int prefix = a.prefix ? a.prefix[it.row] : 0;
-    const int lo_all = a.window ? max(0, r.p0 + 1 - a.window) : 0, t_first = lo_all / 64, t_count = r.skip ? 0 : (total + 63) / 64 - t_first;
+    const int lo_all = a.window ? max(0, r.p0 + 1 - a.window) : 0, t_first = lo_all / TILE, t_count = r.skip ? 0 : (total + TILE - 1) / TILE - t_first;
     const int t0 = t_first + (int)((long long)t_count * it.chunk / it.chunks), t1 = t_first + (int)((long long)t_count * (it.chunk + 1) / it.chunks);
     const int lo_last = a.window ? max(0, total - a.window) : 0, hi_first = min(total, max(r.p0 + 1, prefix));  // what every token sees
     const int* table = a.r.pages + (size_t)it.row * a.r.max_pages;
 
-    v8bf16 qf[NT][KB][2];
+    // The queries as B operands: in registers, or where those are full in LDS (rows spread over the banks by 16 bytes).
+    constexpr bool QL = NT * HD > 512;
+    __shared__ __attribute__((aligned(16))) bf16_t qs[QL ? NT * 16 * (HD + 8) : 8];
+    v8bf16 qf[QL ? 1 : NT][QL ? 1 : KB][2];
+    auto query = [&](int nt, int j, int u) __attribute__((always_inline)) {
+        if constexpr (QL)
+            return *(const v8bf16*)(qs + (nt * 16 + col) * (HD + 8) + j * 64 + g * 16 + u * 8);
+        else
+            return qf[nt][j][u];
+    };
     PagedSight see[NT];
     float slope2[NT], top[NT], sum[NT];
 #pragma unroll
@@ -166,10 +176,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT > 1 ? 1 
         for (int j = 0; j < KB; ++j)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                qf[nt][j][u] = *(const v8bf16*)(qp + j * 64 + u * 8);
-                if (!live) qf[nt][j][u] = (v8bf16)(__bf16)0.0f;
+                v8bf16 x = *(const v8bf16*)(qp + j * 64 + u * 8);
+                if (!live) x = (v8bf16)(__bf16)0.0f;
+                if constexpr (!QL)
+                    qf[nt][j][u] = x;
+                else if (wv == 0)
+                    *(v8bf16*)(qs + row * (HD + 8) + j * 64 + g * 16 + u * 8) = x;
             }
     }
+    if constexpr (QL) __syncthreads();
     v4f o[NT][DB];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -177,123 +192,127 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT > 1 ? 1 
         for (int d = 0; d < DB; ++d) o[nt][d] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
 
     // The pages of a tile's key rows (lane group col / 4 of each block) and of its values (lane group g); -1: none.
-    auto find = [&](int t, int group) { return paged_find(a.r, table, (t * 64 + group * 16) >> shift, a.c.pages); };
-    uint4 kr[4][KB], vr[DB];
+    auto find = [&](int t, int group) { return paged_find(a.r, table, (t * TILE + group * PT) >> shift, a.c.pages); };
+    uint4 kr[NB][KB];
+    words vr[DB];
     float ks, vs;
     auto load_keys = [&](int t, int id) __attribute__((always_inline)) {
         const size_t head = (size_t)max(id, 0) * Hkv + it.kvh;
-        const int slot = (t * 64 + (col >> 2) * 16 + (col & 3)) & (ps - 1);
+        const int slot = (t * TILE + (col >> 2) * PT + (col & 3)) & (ps - 1);
         const uint8_t* p = a.c.k + (head * ps + slot) * HD + g * 16;
         ks = paged_scale(a.c.k_scale[head]);
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
+        for (int j = 0; j < KB; ++j)
 #pragma unroll
-            for (int j = 0; j < KB; ++j) kr[b][j] = *(const uint4*)(p + b * 4 * HD + j * 64);
+            for (int b = 0; b < NB; ++b) kr[b][j] = *(const uint4*)(p + b * 4 * HD + j * 64);
     };
     auto load_values = [&](int t, int id) __attribute__((always_inline)) {
         const size_t head = (size_t)max(id, 0) * Hkv + it.kvh;
-        const uint8_t* p = a.c.v + head * ps * HD + ((size_t)(((t * 64 + g * 16) & (ps - 1)) >> 4) * HD + col) * 16;
+        const int slot = (t * TILE + g * PT) & (ps - 1);
+        const uint8_t* p = a.c.v + head * ps * HD + ((size_t)(slot >> 4) * HD + col) * 16 + (slot & 15);
         vs = paged_scale(a.c.v_scale[head]);
 #pragma unroll
-        for (int d = 0; d < DB; ++d) vr[d] = *(const uint4*)(p + d * 256);
+        for (int d = 0; d < DB; ++d) vr[d] = *(const words*)(p + d * 256);
     };
+    // Loads run a tile ahead (the pages' numbers two), always, so that what is waited for does not depend on the path here:
+    // past its last tile a wave loads that one again.
     int t = t0 + wv;
-    int idk = 0, idv = 0, next_k = 0, next_v = 0;
     if (t < t1) {
-        idk = find(t, col >> 2);
-        idv = find(t, g);
-        if (t + 4 < t1) next_k = find(t + 4, col >> 2), next_v = find(t + 4, g);
+        const int last = t + (t1 - 1 - t) / 4 * 4;
+        int idk = find(t, col >> 2), idv = find(t, g), next_k = find(min(t + 4, last), col >> 2), next_v = find(min(t + 4, last), g);
         load_keys(t, idk);
         load_values(t, idv);
-    }
-    for (; t < t1; t += 4) {
-        float s[NT][16];
-        {
-            v4f c[NT][4];
+        for (; t < t1; t += 4) {
+            float s[NT][PT];
+            {
+                v4f c[NT][NB];
+                const float scale = ks;
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
+                for (int j = 0; j < KB; ++j) {
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int j = 0; j < KB; ++j)
+                    for (int u = 0; u < 2; ++u)
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const v8bf16 kf = u ? paged_widen(kr[b][j].z, kr[b][j].w, ks) : paged_widen(kr[b][j].x, kr[b][j].y, ks);
+                        for (int b = 0; b < NB; ++b) {
+                            const v8bf16 kf = u ? paged_widen(kr[b][j].z, kr[b][j].w, scale) : paged_widen(kr[b][j].x, kr[b][j].y, scale);
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-                            c[nt][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[nt][j][u], j + u ? c[nt][b] : (v4f){0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
-                    }
+                            for (int nt = 0; nt < NT; ++nt)
+                                c[nt][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, query(nt, j, u), j + u ? c[nt][b] : (v4f){0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+                        }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < PT; ++e) s[nt][e] = c[nt][e >> 2][e & 3];
             }
+            const int after_k = find(min(t + 8, last), col >> 2), after_v = find(min(t + 8, last), g);
+            load_keys(min(t + 4, last), next_k);
+            __builtin_amdgcn_sched_barrier(0);
+            const int base = t * TILE, mine = base + g * PT;
+            const bool edge = base < lo_last || base + TILE > hi_first || __any(idv < 0);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt) {
+                paged_scores<PT>(a, s[nt], slope2[nt], mine, see[nt].at);
+                if (edge)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s[nt][e] = c[nt][e >> 2][e & 3];
-        }
-        const bool more = t + 4 < t1;
-        int after_k = 0, after_v = 0;
-        if (more) {
-            if (t + 8 < t1) after_k = find(t + 8, col >> 2), after_v = find(t + 8, g);
-            load_keys(t + 4, next_k);
-        }
-        const int base = t * 64, mine = base + g * 16;
-        const bool edge = base < lo_last || base + 64 > hi_first || __any(idv < 0);
+                    for (int e = 0; e < PT; ++e) s[nt][e] = mine + e < see[nt].lo || mine + e >= see[nt].hi ? -INFINITY : idv < 0 ? QNAN : s[nt][e];
+                float m = s[nt][0];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            paged_scores<16>(a, s[nt], slope2[nt], mine, see[nt].at);
-            if (edge)
+                for (int e = 1; e < PT; ++e) m = fmaxf(m, s[nt][e]);
+                m = fmaxf(m, __shfl_xor(m, 16));
+                m = fmaxf(m, __shfl_xor(m, 32));
+                if (__any(m > top[nt] + SLACK || (top[nt] == -INFINITY && m > -INFINITY))) {
+                    const float up = fmaxf(top[nt], m), f = up == -INFINITY ? 1.0f : exp2_(top[nt] - up);
+                    top[nt] = up;
+                    sum[nt] *= f;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s[nt][e] = mine + e < see[nt].lo || mine + e >= see[nt].hi ? -INFINITY : idv < 0 ? QNAN : s[nt][e];
-            float m = s[nt][0];
+                    for (int d = 0; d < DB; ++d)
 #pragma unroll
-            for (int e = 1; e < 16; ++e) m = fmaxf(m, s[nt][e]);
-            m = fmaxf(m, __shfl_xor(m, 16));
-            m = fmaxf(m, __shfl_xor(m, 32));
-            if (__any(m > top[nt] + SLACK || (top[nt] == -INFINITY && m > -INFINITY))) {
-                const float up = fmaxf(top[nt], m), f = up == -INFINITY ? 1.0f : exp2_(top[nt] - up);
-                top[nt] = up;
-                sum[nt] *= f;
+                        for (int e = 0; e < 4; ++e) o[nt][d][e] *= f;
+                }
+                const float from = top[nt] == -INFINITY ? 0.0f : top[nt];
+#pragma unroll
+                for (int e = 0; e < PT; ++e) {
+                    s[nt][e] = exp2_(s[nt][e] - from);
+                    sum[nt] += s[nt][e];
+                }
+            }
+            if (base + TILE > total || __any(idv < 0)) {  // bytes that no token wrote may be anything
+                const int live = idv < 0 ? 0 : total - mine;
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[nt][d][e] *= f;
+                    for (int x = 0; x < PT / 4; ++x) vr[d][x] &= live >= 4 * x + 4 ? 0xffffffffu : live <= 4 * x ? 0u : (1u << 8 * (live - 4 * x)) - 1;
             }
-            const float from = top[nt] == -INFINITY ? 0.0f : top[nt];
+            v8bf16 pf[NT][PT / 8];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                s[nt][e] = exp2_(s[nt][e] - from);
-                sum[nt] += s[nt][e];
-            }
-        }
-        if (base + 64 > total || __any(idv < 0)) {  // bytes that no token wrote may be anything
-            const int live = idv < 0 ? 0 : total - mine;
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int u = 0; u < PT / 8; ++u) {
+                    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+                    const u4 w = {pk_bf16(s[nt][8 * u], s[nt][8 * u + 1]), pk_bf16(s[nt][8 * u + 2], s[nt][8 * u + 3]),
+                                  pk_bf16(s[nt][8 * u + 4], s[nt][8 * u + 5]), pk_bf16(s[nt][8 * u + 6], s[nt][8 * u + 7])};
+                    pf[nt][u] = __builtin_bit_cast(v8bf16, w);
+                }
+            const float scale = vs;
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
-                uint32_t* w = (uint32_t*)&vr[d];
+                if (d % 4 == 0) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int x = 0; x < 4; ++x) w[x] &= live >= 4 * x + 4 ? 0xffffffffu : live <= 4 * x ? 0u : (1u << 8 * (live - 4 * x)) - 1;
+                for (int u = 0; u < PT / 8; ++u) {
+                    const v8bf16 vf = paged_widen(vr[d][2 * u], vr[d][2 * u + 1], scale);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) o[nt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[nt][u], o[nt][d], 0, 0, 0);
+                }
             }
+            __builtin_amdgcn_sched_barrier(0);
+            load_values(min(t + 4, last), next_v);
+            idk = next_k;
+            idv = next_v;
+            next_k = after_k;
+            next_v = after_v;
         }
-        v8bf16 pf[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-                const u4 w = {pk_bf16(s[nt][8 * u], s[nt][8 * u + 1]), pk_bf16(s[nt][8 * u + 2], s[nt][8 * u + 3]),
-                              pk_bf16(s[nt][8 * u + 4], s[nt][8 * u + 5]), pk_bf16(s[nt][8 * u + 6], s[nt][8 * u + 7])};
-                pf[nt][u] = __builtin_bit_cast(v8bf16, w);
-            }
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const v8bf16 vf = u ? paged_widen(vr[d].z, vr[d].w, vs) : paged_widen(vr[d].x, vr[d].y, vs);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) o[nt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[nt][u], o[nt][d], 0, 0, 0);
-            }
-        if (more) load_values(t + 4, next_v);
-        idk = next_k;
-        idv = next_v;
-        next_k = after_k;
-        next_v = after_v;
     }
 
     // The waves' sums together.
@@ -471,7 +490,7 @@ PagedPlan paged_attention_plan(const PagedCache& c, const PagedRows& r, int q_he
 hipError_t q38_paged_attention(const PagedAttnArgs& a, hipStream_t stream) {
     const int few = a.plan.few, G = a.q_heads / a.c.kv_heads;
     if (a.plan.items) {
-#define STREAM(HD, NT) hipLaunchKernelGGL((paged_stream_kernel<HD, NT>), dim3(a.plan.items), dim3(256), 0, stream, a)
+#define STREAM(HD, NT) hipLaunchKernelGGL((paged_stream_kernel<HD, NT, (HD > 128 ? 8 : 16)>), dim3(a.plan.items), dim3(256), 0, stream, a)
 #define STREAMS(HD)                  \
     switch (few / 16) {              \
         case 1: STREAM(HD, 1); break; \
