@@ -25,7 +25,8 @@ struct PagedPlan {
     int few;                 // rows with at most this many (token, query head) pairs per KV head stream their positions, 16 pairs a tile
     int target;              // workgroups that their positions are cut into, about
     int items, slots;        // workgroups of those at most, and of them those that leave partial sums
-    size_t table, part, bytes;  // places in the scratch: the (row, KV head)s' first slot and count, the partial sums; its size
+    int tiles, cut_slots, cut_jobs, cus;  // workgroups of tiles of query rows; partial sums of cut ones; tiles that may be cut; CUs
+    size_t table, part, cut_part, bytes;  // places in the scratch: the (row, KV head)s' first slot and count, both kinds' partial sums; its size
 };
 PagedPlan paged_attention_plan(const PagedCache& c, const PagedRows& r, int q_heads);
 

@@ -8,6 +8,7 @@
 // The maximum that the weights are relative to is raised, and the sums so far rescaled, only when a score passes it by
 // SLACK: until then weights reach 2^SLACK, which float32 and bf16 hold as exactly as those below one.
 #include <algorithm>
+#include <type_traits>
 
 #include "kernels.h"
 #include "paged.h"
@@ -256,13 +257,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT > 1 ? 1 
                 paged_scores<PT>(a, s[nt], slope2[nt], mine, see[nt].at);
                 if (edge)
 #pragma unroll
-                    for (int e = 0; e < PT; ++e) s[nt][e] = mine + e < see[nt].lo || mine + e >= see[nt].hi ? -INFINITY : idv < 0 ? QNAN : s[nt][e];
+                    for (int e = 0; e < PT; ++e) s[nt][e] = ((mine + e < see[nt].lo) | (mine + e >= see[nt].hi)) ? -INFINITY : idv < 0 ? QNAN : s[nt][e];
                 float m = s[nt][0];
 #pragma unroll
                 for (int e = 1; e < PT; ++e) m = fmaxf(m, s[nt][e]);
                 m = fmaxf(m, __shfl_xor(m, 16));
                 m = fmaxf(m, __shfl_xor(m, 32));
-                if (__any(m > top[nt] + SLACK || (top[nt] == -INFINITY && m > -INFINITY))) {
+                if (__any((m > top[nt] + SLACK) | ((top[nt] == -INFINITY) & (m > -INFINITY)))) {
                     const float up = fmaxf(top[nt], m), f = up == -INFINITY ? 1.0f : exp2_(top[nt] - up);
                     top[nt] = up;
                     sum[nt] *= f;
@@ -391,81 +392,393 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) 
     for (int d = threadIdx.x; d < HD; d += 256) out[d] = f2bf(((sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d])) / all);
 }
 
-template <int E>
-__device__ __forceinline__ void load_dims(const bf16_t* p, float (&x)[E]) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = bf2f(p[e]);
+// ---- Many query rows (prefill chunks): tiles of 256 query rows (tokens x the KV head's query heads) per workgroup.
+//
+// A wave has 64 query rows as two 32-column B operands; keys are A, a sub-block of 32 positions at a time, its rows permuted so
+// that a lane's scores are the eight consecutive positions that it feeds to each step of weights x V, where values are A (a
+// lane then holds four consecutive dims of one query row). Each tile of positions is read from its pages once per workgroup,
+// widened to bf16 by its threads and put into one of three LDS buffers, from which the four waves read it: widening in the
+// waves' own registers would take as long as their MFMAs. 64 rows per wave, because with 32 the waves' LDS reads take as long as
+// their MFMAs (16 KB per 16 MFMAs). Sub-block i + 1's scores go before sub-block i's weights x V, beside whose MFMAs i + 1's weights
+// are formed; the next tile but one is widened beside the scores' MFMAs.
+//
+// Tiles are cut along the positions when they are too few for the CUs (paged_cut): each item's sums then go to scratch in float32
+// (256 KB for heads of 256, as long as a dozen sub-blocks take), and paged_join_tiles_kernel puts them together.
+namespace {
+
+constexpr int PT_ROWS = 64, PT_TILE = 4 * PT_ROWS;
+constexpr int PT_ITEMS = 3;  // items per CU at most when tiles are cut
+constexpr int PT_CUTS = 8;
+
+__device__ __forceinline__ v8bf16 paged_frag(uint32_t at) {
+    return *(const __attribute__((address_space(3))) v8bf16*)(uintptr_t)at;
 }
 
-// A wave per token and query head: its lanes take 64 positions' scores, then, position by position, E dims each.
-template <int E>
-__global__ __launch_bounds__(64) void paged_attention_kernel(const PagedAttnArgs a) {
-    constexpr int HD = E * 64;
-    __shared__ float q[HD];
-    const int lane = threadIdx.x, hq = blockIdx.x % a.q_heads, i = blockIdx.x / a.q_heads % a.r.max_tokens, row = blockIdx.x / a.q_heads / a.r.max_tokens;
-    const int G = a.q_heads / a.c.kv_heads, kvh = hq / G, ps = a.c.page_size;
-    const PagedRow r = paged_row(a.r, row, ps);
-    if (i >= r.n || (a.plan.items && r.n * G <= a.plan.few)) return;
-    const size_t at = ((size_t)(r.t0 + i) * a.q_heads + hq) * HD + lane * E;
-    float o[E] = {}, x[E];
-    float m = -INFINITY, l = 0.0f;
-    if (!r.skip) {
-        load_dims<E>(a.q + at, x);
+// The tiles of the call, and into how many parts each is cut.
+struct PagedTiles {
+    int jobs, cuts;  // (row, tile, KV head)s; parts of each
+};
+
+__device__ __forceinline__ int paged_row_tiles(const PagedAttnArgs& a, int row, int G) {
+    const PagedRow r = paged_row(a.r, row, a.c.page_size);
+    return r.n <= 0 || (a.plan.items && r.n * G <= a.plan.few) ? 0 : (r.n * G + PT_TILE - 1) / PT_TILE;
+}
+
+// Parts that end the last item first when every CU takes items of the longest tile's length / parts, each with about 16
+// sub-blocks' time of its own (queries, first loads, sums).
+__device__ __forceinline__ PagedTiles paged_cut(const PagedAttnArgs& a, int G) {
+    int jobs = 0, longest = 0;
+    for (int row = threadIdx.x & 63; row < a.r.rows; row += 64) {
+        const int n = paged_row_tiles(a, row, G);
+        const PagedRow r = paged_row(a.r, row, a.c.page_size);
+        jobs += n;
+        if (n && !r.skip) longest = max(longest, a.window ? min(r.p0 + r.n, a.window + PT_TILE / G + 64) : r.p0 + r.n);
+    }
 #pragma unroll
-        for (int e = 0; e < E; ++e) q[lane * E + e] = x[e];
-        __syncthreads();
-        const int p = r.p0 + i, total = r.p0 + r.n;
-        const int hi = min(total, max(p + 1, a.prefix ? a.prefix[row] : 0)), lo = a.window ? max(0, p + 1 - a.window) : 0;
-        const float slope = a.slopes ? a.slopes[hq] : 0.0f;
-        const int* table = a.r.pages + (size_t)row * a.r.max_pages;
-        for (int base = lo / 64 * 64; base < hi; base += 64) {
-            const int j = base + lane, id = paged_find(a.r, table, j / ps, a.c.pages);
-            float s = -INFINITY;
-            if (j >= lo && j < hi) {
-                s = QNAN;
-                if (id >= 0) {
-                    const size_t head = (size_t)id * a.c.kv_heads + kvh;
-                    const uint32_t* kp = (const uint32_t*)(a.c.k + (head * ps + j % ps) * HD);
-                    s = 0.0f;
-                    for (int d = 0; d < HD / 4; ++d) {
-                        typedef float v2f_ __attribute__((ext_vector_type(2)));
-                        const uint32_t w = kp[d];
-                        const v2f_ f0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, 1.0f, false), f1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, 1.0f, true);
-                        s += q[d * 4] * f0[0] + q[d * 4 + 1] * f0[1] + q[d * 4 + 2] * f1[0] + q[d * 4 + 3] * f1[1];
-                    }
-                    s *= ldexpf(a.scale, a.c.k_scale[head] - 127);
-                    if (a.cap > 0.0f) s = a.cap * tanhf(s / a.cap);
-                    s += slope * (float)(j - p);
-                }
-            }
-            const float mn = fmaxf(m, warp_max(s)), safe = mn == -INFINITY ? 0.0f : mn, f = expf(m - safe), w = expf(s - safe);
-            m = mn;
-            l = l * f + warp_sum(w);
+    for (int o = 32; o > 0; o >>= 1) jobs += __shfl_xor(jobs, o), longest = max(longest, __shfl_xor(longest, o));
+    jobs *= a.c.kv_heads;
+    longest = (longest + 31) / 32;
+    int cuts = 1, best = 0x7fffffff;
+    for (int c = 1; c <= PT_CUTS && (c == 1 || (jobs * c <= a.plan.cut_slots && longest >= 16 * c)); ++c) {
+        const int cost = ((jobs * c + a.plan.cus - 1) / a.plan.cus) * ((longest + c - 1) / c + 16);
+        if (cost < best) best = cost, cuts = c;
+    }
+    return {jobs, cuts};
+}
+
+// Job j of the call's: its row, its tile in the row (the latest tokens first) and KV head (fastest: the items of one go to
+// the same XCDs, whose L2 then holds its pages).
+struct PagedJob {
+    int row, tile, kvh;
+};
+
+__device__ __forceinline__ PagedJob paged_job(const PagedAttnArgs& a, int j, int G) {
+    const int lane = threadIdx.x & 63, kvh = j % a.c.kv_heads;
+    int left = j / a.c.kv_heads;
+    for (int base = 0; base < a.r.rows; base += 64) {
+        const int n = base + lane < a.r.rows ? paged_row_tiles(a, base + lane, G) : 0;
+        int ends = n;
 #pragma unroll
-            for (int e = 0; e < E; ++e) o[e] *= f;
-            for (int y = 0; y < 64; ++y) {
-                const int jy = base + y;
-                if (jy < lo || jy >= hi) continue;
-                const int idy = __shfl(id, y);
-                const float wy = __shfl(w, y);
-                if (idy < 0) continue;
-                const size_t head = (size_t)idy * a.c.kv_heads + kvh;
-                const float sc = ldexpf(wy, a.c.v_scale[head] - 127);
-                const uint8_t* vp = a.c.v + head * ps * HD + ((size_t)(jy % ps / 16) * HD + lane * E) * 16 + jy % 16;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int x = __shfl_up(ends, o);
+            if (lane >= o) ends += x;
+        }
+        const unsigned long long past = __ballot(ends > left);
+        if (past) {
+            const int l = __ffsll(past) - 1;
+            return {__builtin_amdgcn_readfirstlane(base + l), __builtin_amdgcn_readfirstlane(__shfl(ends, l) - 1 - left), kvh};
+        }
+        left -= __shfl(ends, 63);
+    }
+    return {-1, 0, 0};
+}
+
+}  // namespace
+
+template <int HD>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void paged_tiles_kernel(const PagedAttnArgs a) {
+    constexpr int TILE = 32;                   // positions per LDS buffer
+    constexpr int NI = HD > 128 ? 2 : 1;       // 16-byte pieces of keys, and of values, per thread (heads of 64: of either)
+    constexpr bool EITHER = HD == 64;
+    constexpr int KM = HD / 16, VD = HD / 32, HALF = TILE * HD * 2, BUF = 2 * HALF;  // MFMA steps; bytes of a buffer's keys, of a buffer
+    constexpr int STEPS = EITHER ? 2 : 4 * NI;  // pieces of widening: 8 bf16 each
+    __shared__ __attribute__((aligned(1024))) uint8_t ring[3 * BUF];
+    __shared__ int lost[3][2];
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, h = lane >> 5;
+    const int Hkv = a.c.kv_heads, G = a.q_heads / Hkv, ps = a.c.page_size, shift = __builtin_ctz(ps);
+    const PagedTiles all = paged_cut(a, G);
+    const int z = blockIdx.x / max(all.jobs, 1), j = blockIdx.x % max(all.jobs, 1);
+    if (z >= all.cuts || !all.jobs) return;
+    const PagedJob job = paged_job(a, j, G);
+    if (job.row < 0) return;
+    const PagedRow r = paged_row(a.r, job.row, ps);
+    const int R = r.n * G, total = r.p0 + r.n, prefix = a.prefix ? a.prefix[job.row] : 0;
+    const int first = job.tile * PT_TILE, i_last = min((first + PT_TILE - 1) / G, r.n - 1);  // the tile's first query row, its last token
+    const int* table = a.r.pages + (size_t)job.row * a.r.max_pages;
+
+    // The tiles of positions that any of the workgroup's rows sees; this item's.
+    const int lo_tile = paged_sight(a, r, prefix, first / G).lo / TILE, hi_tile = r.skip ? lo_tile : (paged_sight(a, r, prefix, i_last).hi + TILE - 1) / TILE;
+    const int T0 = lo_tile + (int)((long long)(hi_tile - lo_tile) * z / all.cuts), T1 = lo_tile + (int)((long long)(hi_tile - lo_tile) * (z + 1) / all.cuts);
+
+    const int row0 = first + wv * PT_ROWS;
+    v8bf16 qf[2][KM];
+    PagedSight see[2];
+    float slope2[2], top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f}, from[2] = {0.0f, 0.0f};
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    typedef float v2f_ __attribute__((ext_vector_type(2)));
-                    const v2f_ f0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8((uint32_t)vp[e * 16], 1.0f, false);
-                    o[e] += sc * f0[0];
-                }
-            }
+    for (int rt = 0; rt < 2; ++rt) {
+        const int row = row0 + rt * 32 + l32, i = row / G, head = job.kvh * G + row % G;
+        const bool mine = row < R;
+        see[rt] = mine ? paged_sight(a, r, prefix, i) : PagedSight{0, 0, 0};
+        slope2[rt] = mine && a.slopes ? a.slopes[head] * LOG2E : 0.0f;
+        const bf16_t* qp = a.q + ((size_t)(r.t0 + (mine ? i : 0)) * a.q_heads + (mine ? head : 0)) * HD + h * 8;
+#pragma unroll
+        for (int m = 0; m < KM; ++m) {
+            qf[rt][m] = *(const v8bf16*)(qp + m * 16);
+            if (!mine) qf[rt][m] = (v8bf16)(__bf16)0.0f;
         }
     }
-    const float inv = m == -INFINITY && l == 0.0f ? 0.0f : 1.0f / l;
+    const PagedSight early = paged_sight(a, r, prefix, min(row0, R - 1) / G), late = paged_sight(a, r, prefix, min(row0 + PT_ROWS - 1, R - 1) / G);
+    const int lo_whole = __builtin_amdgcn_readfirstlane(late.lo), hi_whole = __builtin_amdgcn_readfirstlane(early.hi);
+
+    // This thread's pieces of a tile: piece i is position group gi's, 16 dims of one key and 16 positions of one value dim.
+    uint4 rk[NI], rv[NI];
+    int id[NI];
+    float ks[NI], vs[NI];
+    auto load = [&](int T) __attribute__((always_inline)) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) a.out[at + e] = f2bf(o[e] * inv);
+        for (int i = 0; i < NI; ++i) {
+            const int c = EITHER ? threadIdx.x & 127 : threadIdx.x + 256 * i, gi = __builtin_amdgcn_readfirstlane(c / HD), p = T * TILE + gi * 16;
+            id[i] = paged_find(a.r, table, p >> shift, a.c.pages);
+            const size_t head = (size_t)max(id[i], 0) * Hkv + job.kvh, at = (head * ps + (p & (ps - 1))) * HD + (c % HD) * 16;
+            if constexpr (EITHER) {
+                ks[i] = paged_scale((wv < 2 ? a.c.k_scale : a.c.v_scale)[head]);
+                rk[i] = *(const uint4*)((wv < 2 ? a.c.k : a.c.v) + at);
+            } else {
+                ks[i] = paged_scale(a.c.k_scale[head]);
+                vs[i] = paged_scale(a.c.v_scale[head]);
+                rk[i] = *(const uint4*)(a.c.k + at);
+                rv[i] = *(const uint4*)(a.c.v + at);
+            }
+        }
+    };
+    // Step x of widening the loaded tile T into its buffer: half of a piece. Keys: row (position), its 16-byte chunks spread
+    // over the banks; values: per sub-block and dim 32 positions.
+    auto widen = [&](int T, int x) __attribute__((always_inline)) {
+        uint8_t* buf = ring + T % 3 * BUF;
+        const int i = EITHER ? 0 : x >> 2, u = x & 1, c = EITHER ? threadIdx.x & 127 : threadIdx.x + 256 * i;
+        if (EITHER ? wv < 2 : !(x & 2)) {
+            const int p = c / (HD / 16), cc = c % (HD / 16) * 2 + u, spread = HD > 64 ? p & 15 : (p >> 1) & 7;
+            *(v8bf16*)(buf + p * HD * 2 + ((cc ^ spread) << 4)) = u ? paged_widen(rk[i].z, rk[i].w, ks[i]) : paged_widen(rk[i].x, rk[i].y, ks[i]);
+        } else {
+            const uint4 w = EITHER ? rk[i] : rv[i];
+            const int gi = c / HD, d = c % HD, cc = gi * 2 + u, spread = ((d >> 1) & 3) ^ ((d >> 3) & 1);
+            uint32_t w0 = u ? w.z : w.x, w1 = u ? w.w : w.y;
+            const int left = id[i] < 0 ? 0 : total - (T * TILE + gi * 16 + u * 8);
+            if (left < 8) {  // bytes that no token wrote may be anything
+                w0 &= left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << 8 * left) - 1;
+                w1 &= left <= 4 ? 0u : (1u << 8 * (left - 4)) - 1;
+            }
+            *(v8bf16*)(buf + HALF + d * 64 + ((cc ^ spread) << 4)) = paged_widen(w0, w1, EITHER ? ks[i] : vs[i]);
+            if (u && d == 0) lost[T % 3][gi] = id[i] < 0;
+        }
+    };
+
+    const uint32_t lds0 = (uint32_t)(uintptr_t)LDS_PTR(&ring[0]);
+    const int kp = (l32 & ~12) | (l32 & 4) << 1 | (l32 & 8) >> 1;  // the position of this lane's key row
+    const uint32_t kl = kp * HD * 2 + ((h ^ (HD > 64 ? kp & 15 : (kp >> 1) & 7)) << 4);
+    const uint32_t vl = HALF + l32 * 64 + ((h ^ ((l32 >> 1) & 3) ^ ((l32 >> 3) & 1)) << 4);
+    v16f o[2][VD], s[2];
+#pragma unroll
+    for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+        for (int d = 0; d < VD; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[rt][d][e] = 0.0f;
+    typedef uint32_t u4_ __attribute__((ext_vector_type(4)));
+    u4_ pw[2][2];
+    float raise[2] = {1.0f, 1.0f};
+    bool raised = false;
+
+    // Scores of sub-block n (of the call's positions), with tile Tw widened beside them if Tw >= 0; then the maxima.
+    auto scores = [&](int n, auto more) __attribute__((always_inline)) {
+        const uint32_t ka = lds0 + n % 3 * BUF + kl;
+        {
+            v16f zero;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) zero[e] = 0.0f;
+            v8bf16 kf[4];
+#pragma unroll
+            for (int m = 0; m < 4; ++m) kf[m] = paged_frag(ka ^ (m << 5));
+#pragma unroll
+            for (int m = 0; m < KM; ++m) {
+                __builtin_amdgcn_sched_barrier(0);
+                s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[m & 3], qf[0][m], m ? s[0] : zero, 0, 0, 0);
+                s[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[m & 3], qf[1][m], m ? s[1] : zero, 0, 0, 0);
+                if (m + 4 < KM) kf[m & 3] = paged_frag(ka ^ ((m + 4) << 5));
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("" : "+v"(s[0]), "+v"(s[1]));  // in VGPRs, where the weights are formed; the AGPRs hold o
+        }
+        if constexpr (decltype(more)::value) {
+#pragma unroll
+            for (int x = 0; x < STEPS; ++x) widen(n + 1, x);
+        }
+        const int p0 = n * 32;
+        const int* flags = lost[n % 3];
+        const int lost0 = __builtin_amdgcn_readfirstlane(flags[0]), lost1 = __builtin_amdgcn_readfirstlane(flags[1]);
+        const bool whole = (p0 >= lo_whole) & (p0 + 32 <= hi_whole) & !(lost0 | lost1);
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt) {
+            float x[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] = s[rt][e];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {  // the lane's positions: 8 from p0 + 16 k + 8 h on
+                float y[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = x[8 * k + e];
+                paged_scores<8>(a, y, slope2[rt], p0 + 16 * k + 8 * h, see[rt].at);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[8 * k + e] = y[e];
+            }
+            if (!whole)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int p = p0 + 16 * (e >> 3) + 8 * h + (e & 7);
+                    x[e] = (e >> 3 ? lost1 : lost0) ? QNAN : x[e];
+                    x[e] = ((p < see[rt].lo) | (p >= see[rt].hi)) ? -INFINITY : x[e];
+                }
+            float m = x[0];
+#pragma unroll
+            for (int e = 1; e < 16; ++e) m = fmaxf(m, x[e]);
+            m = fmaxf(m, __shfl_xor(m, 32));
+            raise[rt] = 1.0f;
+            if (__any((m > top[rt] + SLACK) | ((top[rt] == -INFINITY) & (m > -INFINITY)))) {
+                const float up = fmaxf(top[rt], m);
+                raise[rt] = up == -INFINITY ? 1.0f : exp2_(top[rt] - up);
+                top[rt] = up;
+                from[rt] = up == -INFINITY ? 0.0f : up;
+                sum[rt] *= raise[rt];
+                raised = true;
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[rt][e] = x[e];
+        }
+    };
+    auto weight2 = [&](int x, u4_ (&w)[2][2]) __attribute__((always_inline)) {
+        const int rt = x >> 3, e = 2 * (x & 7);
+        const float e0 = exp2_(s[rt][e] - from[rt]), e1 = exp2_(s[rt][e + 1] - from[rt]);
+        sum[rt] += e0;
+        sum[rt] += e1;
+        uint32_t both = pk_bf16(e0, e1);
+        asm volatile("" : "+v"(both));  // here, beside the MFMAs, not where it is first used
+        w[rt][(x >> 2) & 1][x & 3] = both;
+    };
+    // Weights x V of sub-block n, beside them the next one's weights.
+    auto values = [&](int n, auto next) __attribute__((always_inline)) {
+        const uint32_t va = lds0 + n % 3 * BUF + vl;
+        auto frag = [&](int x) __attribute__((always_inline)) { return paged_frag((va ^ ((x & 1) << 5)) + (x >> 1) * 2048); };
+        v8bf16 vf[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) vf[x] = frag(x);
+        u4_ nw[2][2];
+#pragma unroll
+        for (int x = 0; x < 2 * VD; ++x) {
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int rt = 0; rt < 2; ++rt)
+                o[rt][x >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[x & 3], __builtin_bit_cast(v8bf16, pw[rt][x & 1]), o[rt][x >> 1], 0, 0, 0);
+            if (x + 4 < 2 * VD) vf[x & 3] = frag(x + 4);
+            if constexpr (decltype(next)::value)
+#pragma unroll
+                for (int y = 0; y < 8 / VD; ++y) weight2(x * (8 / VD) + y, nw);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (decltype(next)::value) {
+#pragma unroll
+            for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+                for (int ks2 = 0; ks2 < 2; ++ks2) pw[rt][ks2] = nw[rt][ks2];
+        }
+    };
+
+    if (T0 < T1) {
+        load(T0);
+#pragma unroll
+        for (int x = 0; x < STEPS; ++x) widen(T0, x);
+        load(min(T0 + 1, T1 - 1));
+#pragma unroll
+        for (int x = 0; x < STEPS; ++x) widen(T0 + 1, x);
+        load(min(T0 + 2, T1 - 1));
+        __syncthreads();
+        // Tile T is in buffer T % 3. A tile is widened into the buffer of the one three before, whose last weights x V every
+        // wave has behind it when it comes to the barrier that a tile begins with.
+        scores(T0, std::false_type{});
+#pragma unroll
+        for (int x = 0; x < 16; ++x) weight2(x, pw);
+        int T = T0;
+        for (;;) {
+            raised = false;
+            while (T + 1 < T1) {
+                __syncthreads();
+                scores(T + 1, std::true_type{});
+                load(min(T + 3, T1 - 1));
+                values(T++, std::true_type{});
+                if (raised) break;
+            }
+            if (!raised) break;
+            // Outside the loop above, so that its path keeps the sums where the MFMAs have them.
+#pragma unroll
+            for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+                for (int d = 0; d < VD; ++d)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[rt][d][e] *= raise[rt];
+        }
+        values(T1 - 1, std::false_type{});
+    }
+
+    if (all.cuts == 1) {
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt) {
+            const float l = sum[rt] + __shfl_xor(sum[rt], 32), inv = r.skip ? 0.0f : 1.0f / l;
+            const int row = row0 + rt * 32 + l32;
+            if (row >= R) continue;
+            bf16_t* out = a.out + ((size_t)(r.t0 + row / G) * a.q_heads + job.kvh * G + row % G) * HD + h * 4;
+#pragma unroll
+            for (int d = 0; d < VD; ++d)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *(uint2*)(out + d * 32 + q * 8) = make_uint2(pk_bf16(o[rt][d][4 * q] * inv, o[rt][d][4 * q + 1] * inv),
+                                                                 pk_bf16(o[rt][d][4 * q + 2] * inv, o[rt][d][4 * q + 3] * inv));
+        }
+        return;
+    }
+    // [item][wave][rt][d][q][lane] of four dims, then per query row its maximum and sum.
+    float* part = (float*)(a.scratch + a.plan.cut_part) + (size_t)(j * all.cuts + z) * (PT_TILE * (HD + 2));
+#pragma unroll
+    for (int rt = 0; rt < 2; ++rt) {
+        const float l = sum[rt] + __shfl_xor(sum[rt], 32);
+        if (h == 0) *(float2*)(part + PT_TILE * HD + (wv * PT_ROWS + rt * 32 + l32) * 2) = make_float2(top[rt], l);
+#pragma unroll
+        for (int d = 0; d < VD; ++d)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                *(v4f*)(part + ((((wv * 2 + rt) * VD + d) * 4 + q) * 64 + lane) * 4) = (v4f){o[rt][d][4 * q], o[rt][d][4 * q + 1], o[rt][d][4 * q + 2], o[rt][d][4 * q + 3]};
+    }
 }
 
+// The parts of cut tiles put together. Grid: jobs x the tile's eight groups of 32 query rows x dims in blocks of 32.
+template <int HD>
+__global__ __launch_bounds__(256) void paged_join_tiles_kernel(const PagedAttnArgs a) {
+    constexpr int VD = HD / 32;
+    const int lane = threadIdx.x & 63, q = threadIdx.x >> 6, l32 = lane & 31, h = lane >> 5;
+    const int Hkv = a.c.kv_heads, G = a.q_heads / Hkv;
+    const PagedTiles all = paged_cut(a, G);
+    const int d = blockIdx.x % VD, group = blockIdx.x / VD % 8, j = blockIdx.x / VD / 8;
+    if (all.cuts == 1 || j >= all.jobs) return;
+    const PagedJob job = paged_job(a, j, G);
+    if (job.row < 0) return;
+    const PagedRow r = paged_row(a.r, job.row, a.c.page_size);
+    const int row = job.tile * PT_TILE + group * 32 + l32;
+    if (row >= r.n * G) return;
+    const size_t step = PT_TILE * (HD + 2);
+    const float* part = (const float*)(a.scratch + a.plan.cut_part) + (size_t)j * all.cuts * step;
+    const float* stats = part + PT_TILE * HD + (group * 32 + l32) * 2;
+    float top = -INFINITY, l = 0.0f;
+    for (int z = 0; z < all.cuts; ++z) top = fmaxf(top, stats[z * step]);
+    v4f o = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+    for (int z = 0; z < all.cuts; ++z) {
+        const float2 s = *(const float2*)(stats + z * step);
+        const float f = s.x == -INFINITY ? (s.y == 0.0f ? 0.0f : 1.0f) : exp2_(s.x - top);
+        l += s.y * f;
+        const v4f v = *(const v4f*)(part + z * step + ((((size_t)group * VD + d) * 4 + q) * 64 + lane) * 4);
+        o += v * f;
+    }
+    const float inv = r.skip ? 0.0f : 1.0f / l;
+    *(uint2*)(a.out + ((size_t)(r.t0 + row / G) * a.q_heads + job.kvh * G + row % G) * HD + d * 32 + q * 8 + h * 4) =
+        make_uint2(pk_bf16(o[0] * inv, o[1] * inv), pk_bf16(o[2] * inv, o[3] * inv));
+}
 
 PagedPlan paged_attention_plan(const PagedCache& c, const PagedRows& r, int q_heads) {
     PagedPlan p{};
@@ -483,6 +796,18 @@ PagedPlan paged_attention_plan(const PagedCache& c, const PagedRows& r, int q_he
         p.table = 0;
         p.part = (size_t)heads * 8 + 255 & ~(size_t)255;
         p.bytes = p.part + (size_t)p.slots * p.few * (c.head_dim + 2) * 4;
+    }
+    if (most > p.few) {
+        const long long jobs = heads * ((most + PT_TILE - 1) / PT_TILE);
+        p.cus = q38_device_cus();
+        // Tiles are cut only while that gives at most PT_ITEMS items per CU, so at most half as many tiles are.
+        const long long longest = (long long)r.max_pages * c.page_size + r.max_tokens;
+        const bool cut = longest >= 2 * 16 * 32 && (r.q_start || jobs * 2 <= PT_ITEMS * p.cus);
+        p.cut_slots = cut ? (int)std::min<long long>(PT_ITEMS * p.cus, jobs * PT_CUTS) : 0;
+        p.cut_jobs = std::min<long long>(p.cut_slots / 2, jobs);
+        p.tiles = (int)std::max<long long>(jobs, p.cut_slots);
+        p.cut_part = p.bytes + 255 & ~(size_t)255;
+        p.bytes = p.cut_part + (size_t)p.cut_slots * PT_TILE * (c.head_dim + 2) * 4;
     }
     return p;
 }
@@ -513,13 +838,17 @@ hipError_t q38_paged_attention(const PagedAttnArgs& a, hipStream_t stream) {
         }
         if ((long long)a.r.max_tokens * G <= few) return hipGetLastError();
     }
-    const size_t grid = (size_t)a.r.rows * a.r.max_tokens * a.q_heads;
-#define ATTEND(E) hipLaunchKernelGGL((paged_attention_kernel<E>), dim3(grid), dim3(64), 0, stream, a)
+#define TILES(HD)                                                                                                             \
+    do {                                                                                                                     \
+        hipLaunchKernelGGL((paged_tiles_kernel<HD>), dim3(a.plan.tiles), dim3(256), 0, stream, a);                           \
+        if (a.plan.cut_slots) hipLaunchKernelGGL((paged_join_tiles_kernel<HD>), dim3(a.plan.cut_jobs * 8 * (HD / 32)), dim3(256), 0, stream, a); \
+    } while (0)
     switch (a.c.head_dim) {
-        case 64: ATTEND(1); break;
-        case 128: ATTEND(2); break;
-        case 256: ATTEND(4); break;
+        case 64: TILES(64); break;
+        case 128: TILES(128); break;
+        case 256: TILES(256); break;
         default: return hipErrorInvalidValue;
     }
+#undef TILES
     return hipGetLastError();
 }
