@@ -319,7 +319,7 @@ typedef struct q38_paged_tokens {
 int q38_paged_append(const q38_paged_cache* cache, const q38_paged_rows* rows, const q38_paged_tokens* tokens, void* stream);
 
 /* Queries and options of q38_paged_attention: q, out bf16 [tokens][q_heads][head_dim] (16-byte aligned; query head h reads KV
- * head h / (q_heads / kv_heads), at most 64 to one). The score of position j for the token at position i is scale * q . k_j, then
+ * head h / (q_heads / kv_heads), at most 64 to one). The score of position j for the token at position i is scale * q . k_j (scale > 0), then
  * with cap > 0 cap * tanh(score / cap), then with slopes (float32 [q_heads]) + slope * (j - i). The token sees the positions up
  * to its own, of them with window > 0 the last `window`; with prefix (int32 [rows]) also those below prefix[row], later tokens of
  * the call included. A window and a prefix exclude each other. */

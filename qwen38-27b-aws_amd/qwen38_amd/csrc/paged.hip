@@ -324,7 +324,7 @@ int q38_paged_attention(const q38_paged_cache* c, const q38_paged_rows* r, const
     if (!q || !q->q || !q->out) return q38_report("null argument");
     if (q->q_heads < 1 || q->q_heads % c->kv_heads || q->q_heads / c->kv_heads > 64)
         return q38_report("paged attention: q_heads must be 1 to 64 times kv_heads");
-    if (!(q->scale > -INFINITY && q->scale < INFINITY)) return q38_report("paged attention: scale must be finite");
+    if (!(q->scale > 0.0f && q->scale < INFINITY)) return q38_report("paged attention: scale must be positive and finite");
     if (!(q->cap >= 0.0f && q->cap < INFINITY)) return q38_report("paged attention: cap must be finite and not negative");
     if (q->window < 0) return q38_report("paged attention: window must not be negative");
     if (q->window && q->prefix) return q38_report("paged attention: a window and a prefix exclude each other");

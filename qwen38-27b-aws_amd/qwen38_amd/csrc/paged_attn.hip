@@ -17,6 +17,14 @@ namespace {
 
 constexpr float LOG2E = 1.44269504088896340736f, SLACK = 8.0f;
 
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// A workgroup's row: the same in every lane, and known to be.
+__device__ __forceinline__ PagedRow paged_row_uniform(const PagedRows& a, int row, int page_size) {
+    const PagedRow r = paged_row(a, row, page_size);
+    return {uniform(r.t0), uniform(r.n), uniform(r.p0), uniform(r.skip) != 0};
+}
+
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // What a packed query row (token r / G, query head r % G of the KV head's G) sees: positions [lo, hi); at is its own.
@@ -138,15 +146,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT > 1 ? 1 
     const int Hkv = a.c.kv_heads, G = a.q_heads / Hkv, ps = a.c.page_size, shift = __builtin_ctz(ps);
     PagedItem it;
     if (!paged_item(a, blockIdx.x, G, a.plan.target, it)) return;
-    it.row = __builtin_amdgcn_readfirstlane(it.row);
-    it.kvh = __builtin_amdgcn_readfirstlane(it.kvh);
-    const PagedRow r = paged_row(a.r, it.row, ps);
+    it = {uniform(it.row), uniform(it.kvh), uniform(it.chunk), uniform(it.chunks), uniform(it.slot)};
+    const PagedRow r = paged_row_uniform(a.r, it.row, ps);
     const int R = r.n * G, total = r.p0 + r.n;
     if (it.chunk == 0 && threadIdx.x == 0) {
         int2* t = (int2*)(a.scratch + a.plan.table);
         t[it.row * Hkv + it.kvh] = make_int2(it.slot, it.chunks);
     }
-    const int prefix = a.prefix ? a.prefix[it.row] : 0;
+    const int prefix = a.prefix ? uniform(a.prefix[it.row]) : 0;
     const int lo_all = a.window ? max(0, r.p0 + 1 - a.window) : 0, t_first = lo_all / TILE, t_count = r.skip ? 0 : (total + TILE - 1) / TILE - t_first;
     const int t0 = t_first + (int)((long long)t_count * it.chunk / it.chunks), t1 = t_first + (int)((long long)t_count * (it.chunk + 1) / it.chunks);
     const int lo_last = a.window ? max(0, total - a.window) : 0, hi_first = min(total, max(r.p0 + 1, prefix));  // what every token sees
@@ -443,7 +450,7 @@ __device__ __forceinline__ PagedTiles paged_cut(const PagedAttnArgs& a, int G) {
         const int cost = ((jobs * c + a.plan.cus - 1) / a.plan.cus) * ((longest + c - 1) / c + 16);
         if (cost < best) best = cost, cuts = c;
     }
-    return {jobs, cuts};
+    return {__builtin_amdgcn_readfirstlane(jobs), __builtin_amdgcn_readfirstlane(cuts)};
 }
 
 // Job j of the call's: its row, its tile in the row (the latest tokens first) and KV head (fastest: the items of one go to
@@ -466,7 +473,7 @@ __device__ __forceinline__ PagedJob paged_job(const PagedAttnArgs& a, int j, int
         const unsigned long long past = __ballot(ends > left);
         if (past) {
             const int l = __ffsll(past) - 1;
-            return {__builtin_amdgcn_readfirstlane(base + l), __builtin_amdgcn_readfirstlane(__shfl(ends, l) - 1 - left), kvh};
+            return {uniform(base + l), uniform(__shfl(ends, l) - 1 - left), kvh};
         }
         left -= __shfl(ends, 63);
     }
@@ -481,6 +488,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     constexpr int NI = HD > 128 ? 2 : 1;       // 16-byte pieces of keys, and of values, per thread (heads of 64: of either)
     constexpr bool EITHER = HD == 64;
     constexpr int KM = HD / 16, VD = HD / 32, HALF = TILE * HD * 2, BUF = 2 * HALF;  // MFMA steps; bytes of a buffer's keys, of a buffer
+    constexpr int DEEP = HD > 128 ? 3 : 4;     // operands read ahead from LDS
     constexpr int STEPS = EITHER ? 2 : 4 * NI;  // pieces of widening: 8 bf16 each
     __shared__ __attribute__((aligned(1024))) uint8_t ring[3 * BUF];
     __shared__ int lost[3][2];
@@ -491,8 +499,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     if (z >= all.cuts || !all.jobs) return;
     const PagedJob job = paged_job(a, j, G);
     if (job.row < 0) return;
-    const PagedRow r = paged_row(a.r, job.row, ps);
-    const int R = r.n * G, total = r.p0 + r.n, prefix = a.prefix ? a.prefix[job.row] : 0;
+    const PagedRow r = paged_row_uniform(a.r, job.row, ps);
+    const int R = r.n * G, total = r.p0 + r.n, prefix = a.prefix ? uniform(a.prefix[job.row]) : 0;
     const int first = job.tile * PT_TILE, i_last = min((first + PT_TILE - 1) / G, r.n - 1);  // the tile's first query row, its last token
     const int* table = a.r.pages + (size_t)job.row * a.r.max_pages;
 
@@ -502,14 +510,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
 
     const int row0 = first + wv * PT_ROWS;
     v8bf16 qf[2][KM];
-    PagedSight see[2];
-    float slope2[2], top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f}, from[2] = {0.0f, 0.0f};
+    int token[2];  // of this lane's query rows; -1: none
+    __shared__ float slopes[PT_TILE];
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {
         const int row = row0 + rt * 32 + l32, i = row / G, head = job.kvh * G + row % G;
         const bool mine = row < R;
-        see[rt] = mine ? paged_sight(a, r, prefix, i) : PagedSight{0, 0, 0};
-        slope2[rt] = mine && a.slopes ? a.slopes[head] * LOG2E : 0.0f;
+        token[rt] = mine ? i : -1;
+        if (h == 0) slopes[wv * PT_ROWS + rt * 32 + l32] = mine && a.slopes ? a.slopes[head] * LOG2E : 0.0f;
         const bf16_t* qp = a.q + ((size_t)(r.t0 + (mine ? i : 0)) * a.q_heads + (mine ? head : 0)) * HD + h * 8;
 #pragma unroll
         for (int m = 0; m < KM; ++m) {
@@ -518,136 +526,164 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
         }
     }
     const PagedSight early = paged_sight(a, r, prefix, min(row0, R - 1) / G), late = paged_sight(a, r, prefix, min(row0 + PT_ROWS - 1, R - 1) / G);
-    const int lo_whole = __builtin_amdgcn_readfirstlane(late.lo), hi_whole = __builtin_amdgcn_readfirstlane(early.hi);
+    const int lo_whole = uniform(late.lo), hi_whole = uniform(early.hi);
 
     // This thread's pieces of a tile: piece i is position group gi's, 16 dims of one key and 16 positions of one value dim.
     uint4 rk[NI], rv[NI];
-    int id[NI];
-    float ks[NI], vs[NI];
+    int id[NI], found[NI], ks[NI], vs[NI];  // this tile's pages; the next one's as read; scale bytes
+    const int c0 = EITHER ? threadIdx.x & 127 : threadIdx.x, vg0 = uniform(c0 / HD);
+    // A tile's page numbers are read a tile before its keys and values, so that no load waits for another.
+    auto look = [&](int T) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int page = (T * TILE + (vg0 + i) * 16) >> shift;
+            found[i] = page < a.r.max_pages ? table[page] : -1;
+        }
+    };
     auto load = [&](int T) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            const int c = EITHER ? threadIdx.x & 127 : threadIdx.x + 256 * i, gi = __builtin_amdgcn_readfirstlane(c / HD), p = T * TILE + gi * 16;
-            id[i] = paged_find(a.r, table, p >> shift, a.c.pages);
-            const size_t head = (size_t)max(id[i], 0) * Hkv + job.kvh, at = (head * ps + (p & (ps - 1))) * HD + (c % HD) * 16;
+            id[i] = uniform(found[i]);
+            id[i] = id[i] < a.c.pages ? id[i] : -1;
+            const size_t head = (size_t)max(id[i], 0) * Hkv + job.kvh, at = (head * ps + ((T * TILE + (vg0 + i) * 16) & (ps - 1))) * HD;
             if constexpr (EITHER) {
-                ks[i] = paged_scale((wv < 2 ? a.c.k_scale : a.c.v_scale)[head]);
-                rk[i] = *(const uint4*)((wv < 2 ? a.c.k : a.c.v) + at);
+                ks[i] = (wv < 2 ? a.c.k_scale : a.c.v_scale)[head];
+                rk[i] = *(const uint4*)((wv < 2 ? a.c.k : a.c.v) + at + c0 % HD * 16);
             } else {
-                ks[i] = paged_scale(a.c.k_scale[head]);
-                vs[i] = paged_scale(a.c.v_scale[head]);
-                rk[i] = *(const uint4*)(a.c.k + at);
-                rv[i] = *(const uint4*)(a.c.v + at);
+                ks[i] = a.c.k_scale[head];
+                vs[i] = a.c.v_scale[head];
+                rk[i] = *(const uint4*)(a.c.k + at + c0 % HD * 16);
+                rv[i] = *(const uint4*)(a.c.v + at + c0 % HD * 16);
             }
         }
     };
     // Step x of widening the loaded tile T into its buffer: half of a piece. Keys: row (position), its 16-byte chunks spread
-    // over the banks; values: per sub-block and dim 32 positions.
+    // over the banks; values: per dim 32 positions, likewise.
+    const uint32_t lds0 = (uint32_t)(uintptr_t)LDS_PTR(&ring[0]);
+    const int kp0 = c0 / (HD / 16), kc0 = c0 % (HD / 16) * 2, vd0 = c0 % HD;
+    const uint32_t put_k = kp0 * HD * 2 + ((kc0 ^ (HD > 64 ? kp0 & 15 : (kp0 >> 1) & 7)) << 4);
+    const uint32_t put_v = HALF + vd0 * 64 + ((vg0 * 2 ^ ((vd0 >> 1) & 3) ^ ((vd0 >> 3) & 1)) << 4);
+    auto put = [&](uint32_t at, v8bf16 x) __attribute__((always_inline)) { *(__attribute__((address_space(3))) v8bf16*)(uintptr_t)at = x; };
     auto widen = [&](int T, int x) __attribute__((always_inline)) {
-        uint8_t* buf = ring + T % 3 * BUF;
-        const int i = EITHER ? 0 : x >> 2, u = x & 1, c = EITHER ? threadIdx.x & 127 : threadIdx.x + 256 * i;
-        if (EITHER ? wv < 2 : !(x & 2)) {
-            const int p = c / (HD / 16), cc = c % (HD / 16) * 2 + u, spread = HD > 64 ? p & 15 : (p >> 1) & 7;
-            *(v8bf16*)(buf + p * HD * 2 + ((cc ^ spread) << 4)) = u ? paged_widen(rk[i].z, rk[i].w, ks[i]) : paged_widen(rk[i].x, rk[i].y, ks[i]);
-        } else {
-            const uint4 w = EITHER ? rk[i] : rv[i];
-            const int gi = c / HD, d = c % HD, cc = gi * 2 + u, spread = ((d >> 1) & 3) ^ ((d >> 3) & 1);
-            uint32_t w0 = u ? w.z : w.x, w1 = u ? w.w : w.y;
-            const int left = id[i] < 0 ? 0 : total - (T * TILE + gi * 16 + u * 8);
-            if (left < 8) {  // bytes that no token wrote may be anything
-                w0 &= left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << 8 * left) - 1;
-                w1 &= left <= 4 ? 0u : (1u << 8 * (left - 4)) - 1;
+        const uint32_t buf = lds0 + T % 3 * BUF;
+        const int i = EITHER ? 0 : x >> 2, u = x & 1;
+        if (x == 0) {
+            // Bytes that no token wrote may be anything, and so may those of a page that is not there.
+            bool tail = T * TILE + TILE > total;
+#pragma unroll
+            for (int k = 0; k < NI; ++k) tail |= id[k] < 0;
+            if (tail) {
+#pragma unroll
+                for (int k = 0; k < NI; ++k) {
+                    const int left = id[k] < 0 ? 0 : total - (T * TILE + (vg0 + k) * 16);
+                    uint32_t* w = (uint32_t*)(EITHER ? &rk[k] : &rv[k]);
+                    if (!EITHER || wv >= 2)
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) w[y] &= left >= 4 * y + 4 ? 0xffffffffu : left <= 4 * y ? 0u : (1u << 8 * (left - 4 * y)) - 1;
+                }
             }
-            *(v8bf16*)(buf + HALF + d * 64 + ((cc ^ spread) << 4)) = paged_widen(w0, w1, EITHER ? ks[i] : vs[i]);
-            if (u && d == 0) lost[T % 3][gi] = id[i] < 0;
+#pragma unroll
+            for (int k = 0; k < NI; ++k)
+                if (vd0 == 0) lost[T % 3][vg0 + k] = id[k] < 0;
         }
+        if (EITHER ? wv < 2 : !(x & 2))
+            put(buf + i * (256 / (HD / 16) * HD * 2) + (put_k ^ (u << 4)), u ? paged_widen(rk[i].z, rk[i].w, paged_scale(ks[i])) : paged_widen(rk[i].x, rk[i].y, paged_scale(ks[i])));
+        else if constexpr (EITHER)
+            put(buf + (put_v ^ (u << 4)), u ? paged_widen(rk[0].z, rk[0].w, paged_scale(ks[0])) : paged_widen(rk[0].x, rk[0].y, paged_scale(ks[0])));
+        else
+            put(buf + (put_v ^ (i << 5) ^ (u << 4)), u ? paged_widen(rv[i].z, rv[i].w, paged_scale(vs[i])) : paged_widen(rv[i].x, rv[i].y, paged_scale(vs[i])));
     };
 
-    const uint32_t lds0 = (uint32_t)(uintptr_t)LDS_PTR(&ring[0]);
     const int kp = (l32 & ~12) | (l32 & 4) << 1 | (l32 & 8) >> 1;  // the position of this lane's key row
     const uint32_t kl = kp * HD * 2 + ((h ^ (HD > 64 ? kp & 15 : (kp >> 1) & 7)) << 4);
     const uint32_t vl = HALF + l32 * 64 + ((h ^ ((l32 >> 1) & 3) ^ ((l32 >> 3) & 1)) << 4);
     v16f o[2][VD], s[2];
-#pragma unroll
-    for (int rt = 0; rt < 2; ++rt)
-#pragma unroll
-        for (int d = 0; d < VD; ++d)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[rt][d][e] = 0.0f;
     typedef uint32_t u4_ __attribute__((ext_vector_type(4)));
     u4_ pw[2][2];
-    float raise[2] = {1.0f, 1.0f};
-    bool raised = false;
+    // Scores in powers of two: times scale log2 e beside the exponential, or capped and biased (`bent`) before the maxima.
+    const bool bent = a.cap > 0.0f || a.slopes;
+    const float mul = bent ? 1.0f : a.scale * LOG2E;
+    // What a query row's weights are relative to is the largest score of the first sub-block that it sees anything of, and
+    // stays: floats hold weights of up to 2^LEAP as exactly as others. Only if some score leaps further than that are the item's
+    // sums formed again, relative to the largest score, which is known by then. (Raising it on the way costs the loop
+    // copies of the sums even where it never happens: the compiler keeps them out of the MFMAs' registers for it.)
+    constexpr float LEAP = 40.0f, UNSEEN = -3e38f;
+    float top[2] = {UNSEEN, UNSEEN}, most[2] = {-INFINITY, -INFINITY}, sum[2];
 
-    // Scores of sub-block n (of the call's positions), with tile Tw widened beside them if Tw >= 0; then the maxima.
+    // Scores of sub-block n, with the loaded tile (n + 1) widened beside their MFMAs; then what the weights are relative to.
     auto scores = [&](int n, auto more) __attribute__((always_inline)) {
         const uint32_t ka = lds0 + n % 3 * BUF + kl;
-        {
-            v16f zero;
+        v8bf16 kf[DEEP];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) zero[e] = 0.0f;
-            v8bf16 kf[4];
+        for (int m = 0; m < DEEP; ++m) kf[m] = paged_frag(ka ^ (m << 5));
 #pragma unroll
-            for (int m = 0; m < 4; ++m) kf[m] = paged_frag(ka ^ (m << 5));
-#pragma unroll
-            for (int m = 0; m < KM; ++m) {
-                __builtin_amdgcn_sched_barrier(0);
-                s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[m & 3], qf[0][m], m ? s[0] : zero, 0, 0, 0);
-                s[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[m & 3], qf[1][m], m ? s[1] : zero, 0, 0, 0);
-                if (m + 4 < KM) kf[m & 3] = paged_frag(ka ^ ((m + 4) << 5));
-            }
+        for (int m = 0; m < KM; ++m) {
             __builtin_amdgcn_sched_barrier(0);
-            asm volatile("" : "+v"(s[0]), "+v"(s[1]));  // in VGPRs, where the weights are formed; the AGPRs hold o
+            if (m)
+                asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %2, %3, %0\n\tv_mfma_f32_32x32x16_bf16 %1, %2, %4, %1"
+                             : "+v"(s[0]), "+v"(s[1]) : "v"(kf[m % DEEP]), "v"(qf[0][m]), "v"(qf[1][m]));
+            else
+                asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %2, %3, 0\n\tv_mfma_f32_32x32x16_bf16 %1, %2, %4, 0"
+                             : "=&v"(s[0]), "=&v"(s[1]) : "v"(kf[m % DEEP]), "v"(qf[0][m]), "v"(qf[1][m]));
+            if (m + DEEP < KM) kf[m % DEEP] = paged_frag(ka ^ ((m + DEEP) << 5));
+            if constexpr (decltype(more)::value)
+                if (m >= KM - STEPS) widen(n + 1, m - (KM - STEPS));
         }
-        if constexpr (decltype(more)::value) {
-#pragma unroll
-            for (int x = 0; x < STEPS; ++x) widen(n + 1, x);
+        if constexpr (decltype(more)::value) {  // as early as the registers are free again: a tile's time before they are widened
+            load(min(n + 2, T1 - 1));
+            look(min(n + 3, T1 - 1));
         }
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_nop 15\n\ts_nop 15" : "+v"(s[0]), "+v"(s[1]));  // the last products' way into the registers
         const int p0 = n * 32;
-        const int* flags = lost[n % 3];
-        const int lost0 = __builtin_amdgcn_readfirstlane(flags[0]), lost1 = __builtin_amdgcn_readfirstlane(flags[1]);
-        const bool whole = (p0 >= lo_whole) & (p0 + 32 <= hi_whole) & !(lost0 | lost1);
+        const int lost0 = uniform(lost[n % 3][0]), lost1 = uniform(lost[n % 3][1]);
+        if (bent) {
 #pragma unroll
-        for (int rt = 0; rt < 2; ++rt) {
-            float x[16];
+            for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) x[e] = s[rt][e];
+                for (int k = 0; k < 2; ++k) {  // the lane's positions: 8 from p0 + 16 k + 8 h on
+                    float y[8];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {  // the lane's positions: 8 from p0 + 16 k + 8 h on
-                float y[8];
+                    for (int e = 0; e < 8; ++e) y[e] = s[rt][8 * k + e];
+                    paged_scores<8>(a, y, slopes[wv * PT_ROWS + rt * 32 + l32], p0 + 16 * k + 8 * h, r.p0 + token[rt]);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = x[8 * k + e];
-                paged_scores<8>(a, y, slope2[rt], p0 + 16 * k + 8 * h, see[rt].at);
+                    for (int e = 0; e < 8; ++e) s[rt][8 * k + e] = y[e];
+                }
+        }
+        if (!((p0 >= lo_whole) & (p0 + 32 <= hi_whole) & !(lost0 | lost1))) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[8 * k + e] = y[e];
-            }
-            if (!whole)
+            for (int rt = 0; rt < 2; ++rt) {
+                const PagedSight see = paged_sight(a, r, prefix, max(token[rt], 0));
+                const int lo = see.lo - p0 - 8 * h, hi = token[rt] < 0 ? -64 : see.hi - p0 - 8 * h;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const int p = p0 + 16 * (e >> 3) + 8 * h + (e & 7);
-                    x[e] = (e >> 3 ? lost1 : lost0) ? QNAN : x[e];
-                    x[e] = ((p < see[rt].lo) | (p >= see[rt].hi)) ? -INFINITY : x[e];
+                    const int p = 16 * (e >> 3) + (e & 7);
+                    const float x = (e >> 3 ? lost1 : lost0) ? QNAN : s[rt][e];
+                    s[rt][e] = ((p < lo) | (p >= hi)) ? -INFINITY : x;
                 }
-            float m = x[0];
-#pragma unroll
-            for (int e = 1; e < 16; ++e) m = fmaxf(m, x[e]);
-            m = fmaxf(m, __shfl_xor(m, 32));
-            raise[rt] = 1.0f;
-            if (__any((m > top[rt] + SLACK) | ((top[rt] == -INFINITY) & (m > -INFINITY)))) {
-                const float up = fmaxf(top[rt], m);
-                raise[rt] = up == -INFINITY ? 1.0f : exp2_(top[rt] - up);
-                top[rt] = up;
-                from[rt] = up == -INFINITY ? 0.0f : up;
-                sum[rt] *= raise[rt];
-                raised = true;
             }
+        }
+        // Of seen scores; NaN ones are passed over.
+        auto max3 = [](float x, float y, float z) __attribute__((always_inline)) {
+            float m;
+            asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(x), "v"(y), "v"(z));
+            return m;
+        };
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[rt][e] = x[e];
+        for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) most[rt] = max3(s[rt][e], s[rt][e + 1], most[rt]);
+        if (__any((top[0] == UNSEEN) | (top[1] == UNSEEN))) {
+#pragma unroll
+            for (int rt = 0; rt < 2; ++rt) {
+                const float m = fmaxf(most[rt], __shfl_xor(most[rt], 32)) * mul;
+                top[rt] = ((top[rt] == UNSEEN) & (m > -INFINITY)) ? m : top[rt];
+            }
         }
     };
     auto weight2 = [&](int x, u4_ (&w)[2][2]) __attribute__((always_inline)) {
         const int rt = x >> 3, e = 2 * (x & 7);
-        const float e0 = exp2_(s[rt][e] - from[rt]), e1 = exp2_(s[rt][e + 1] - from[rt]);
+        const float e0 = exp2_(__builtin_fmaf(s[rt][e], mul, -top[rt])), e1 = exp2_(__builtin_fmaf(s[rt][e + 1], mul, -top[rt]));
         sum[rt] += e0;
         sum[rt] += e1;
         uint32_t both = pk_bf16(e0, e1);
@@ -658,17 +694,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     auto values = [&](int n, auto next) __attribute__((always_inline)) {
         const uint32_t va = lds0 + n % 3 * BUF + vl;
         auto frag = [&](int x) __attribute__((always_inline)) { return paged_frag((va ^ ((x & 1) << 5)) + (x >> 1) * 2048); };
-        v8bf16 vf[4];
+        v8bf16 vf[DEEP];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) vf[x] = frag(x);
+        for (int x = 0; x < DEEP; ++x) vf[x] = frag(x);
         u4_ nw[2][2];
 #pragma unroll
         for (int x = 0; x < 2 * VD; ++x) {
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int rt = 0; rt < 2; ++rt)
-                o[rt][x >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[x & 3], __builtin_bit_cast(v8bf16, pw[rt][x & 1]), o[rt][x >> 1], 0, 0, 0);
-            if (x + 4 < 2 * VD) vf[x & 3] = frag(x + 4);
+                o[rt][x >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[x % DEEP], __builtin_bit_cast(v8bf16, pw[rt][x & 1]), o[rt][x >> 1], 0, 0, 0);
+            if (x + DEEP < 2 * VD) vf[x % DEEP] = frag(x + DEEP);
             if constexpr (decltype(next)::value)
 #pragma unroll
                 for (int y = 0; y < 8 / VD; ++y) weight2(x * (8 / VD) + y, nw);
@@ -682,40 +718,48 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
         }
     };
 
-    if (T0 < T1) {
+    for (int pass = 0;; ++pass) {
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt) {
+            sum[rt] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < VD; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[rt][d][e] = 0.0f;
+        }
+        if (T0 >= T1) break;
+        look(T0);
         load(T0);
+        look(min(T0 + 1, T1 - 1));
 #pragma unroll
         for (int x = 0; x < STEPS; ++x) widen(T0, x);
         load(min(T0 + 1, T1 - 1));
+        look(min(T0 + 2, T1 - 1));
 #pragma unroll
         for (int x = 0; x < STEPS; ++x) widen(T0 + 1, x);
         load(min(T0 + 2, T1 - 1));
+        look(min(T0 + 3, T1 - 1));
         __syncthreads();
         // Tile T is in buffer T % 3. A tile is widened into the buffer of the one three before, whose last weights x V every
         // wave has behind it when it comes to the barrier that a tile begins with.
         scores(T0, std::false_type{});
 #pragma unroll
         for (int x = 0; x < 16; ++x) weight2(x, pw);
-        int T = T0;
-        for (;;) {
-            raised = false;
-            while (T + 1 < T1) {
-                __syncthreads();
-                scores(T + 1, std::true_type{});
-                load(min(T + 3, T1 - 1));
-                values(T++, std::true_type{});
-                if (raised) break;
-            }
-            if (!raised) break;
-            // Outside the loop above, so that its path keeps the sums where the MFMAs have them.
-#pragma unroll
-            for (int rt = 0; rt < 2; ++rt)
-#pragma unroll
-                for (int d = 0; d < VD; ++d)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) o[rt][d][e] *= raise[rt];
+        for (int T = T0; T + 1 < T1; ++T) {
+            __syncthreads();
+            scores(T + 1, std::true_type{});
+            values(T, std::true_type{});
         }
         values(T1 - 1, std::false_type{});
+        bool leapt = false;
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt) {
+            most[rt] = fmaxf(most[rt], __shfl_xor(most[rt], 32)) * mul;
+            leapt |= most[rt] > top[rt] + LEAP;
+        }
+        if (pass || !__syncthreads_or(leapt)) break;
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt) top[rt] = fmaxf(top[rt], most[rt]);
     }
 
     if (all.cuts == 1) {
@@ -770,7 +814,7 @@ __global__ __launch_bounds__(256) void paged_join_tiles_kernel(const PagedAttnAr
     v4f o = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
     for (int z = 0; z < all.cuts; ++z) {
         const float2 s = *(const float2*)(stats + z * step);
-        const float f = s.x == -INFINITY ? (s.y == 0.0f ? 0.0f : 1.0f) : exp2_(s.x - top);
+        const float f = s.x == top ? 1.0f : exp2_(s.x - top);  // the same where no part saw anything, or only NaN
         l += s.y * f;
         const v4f v = *(const v4f*)(part + z * step + ((((size_t)group * VD + d) * 4 + q) * 64 + lane) * 4);
         o += v * f;

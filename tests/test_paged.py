@@ -67,7 +67,7 @@ def test_append_refuses(changes, message):
 
 @pytest.mark.parametrize("changes, message", [
     ({"q__q": None}, "null"), ({"q__out": None}, "null"), ({"q__q_heads": 5}, "q_heads"), ({"q__q_heads": 130}, "q_heads"), ({"q__q_heads": 0}, "q_heads"),
-    ({"q__scale": float("nan")}, "scale"), ({"q__scale": float("inf")}, "scale"), ({"q__cap": -1.0}, "cap"), ({"q__cap": float("inf")}, "cap"),
+    ({"q__scale": float("nan")}, "scale"), ({"q__scale": float("inf")}, "scale"), ({"q__scale": 0.0}, "scale"), ({"q__scale": -1.0}, "scale"), ({"q__cap": -1.0}, "cap"), ({"q__cap": float("inf")}, "cap"),
     ({"q__window": -1}, "window"), ({"q__window": 4, "q__prefix": P}, "exclude"), ({"q__out": P + 8}, "aligned"),
 ])
 def test_attention_refuses(changes, message):
