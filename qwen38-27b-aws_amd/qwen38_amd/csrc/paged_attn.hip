@@ -102,15 +102,16 @@ __device__ __forceinline__ int paged_units(const PagedAttnArgs& a, int row, int 
 
 __device__ __forceinline__ bool paged_item(const PagedAttnArgs& a, int id, int G, int target, PagedItem& it) {
     const int lane = threadIdx.x & 63, Hkv = a.c.kv_heads;
-    double total = 0.0;
-    for (int row = lane; row < a.r.rows; row += 64) total += paged_units(a, row, G);
+    const int units0 = lane < a.r.rows ? paged_units(a, lane, G) : 0;  // of the first 64 rows, for both rounds
+    double total = units0;
+    for (int row = lane + 64; row < a.r.rows; row += 64) total += paged_units(a, row, G);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
     const int per = max(1, (int)((total * Hkv + (target - 1)) / target));
     int before = 0, slots = 0;  // items and slots of the rows so far
     for (int base = 0; base < a.r.rows; base += 64) {
         const int row = base + lane;
-        const int n = row < a.r.rows ? (paged_units(a, row, G) + per - 1) / per : 0, m = n > 1 ? n : 0;
+        const int units = base == 0 ? units0 : row < a.r.rows ? paged_units(a, row, G) : 0, n = (units + per - 1) / per, m = n > 1 ? n : 0;
         int ends = n, slot_ends = m;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -409,81 +410,133 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) 
 // their MFMAs (16 KB per 16 MFMAs). Sub-block i + 1's scores go before sub-block i's weights x V, beside whose MFMAs i + 1's weights
 // are formed; the next tile but one is widened beside the scores' MFMAs.
 //
-// Tiles are cut along the positions when they are too few for the CUs (paged_cut): each item's sums then go to scratch in float32
-// (256 KB for heads of 256, as long as a dozen sub-blocks take), and paged_join_tiles_kernel puts them together.
+// While tiles are few, the sub-blocks of all of them, one after another, are dealt out to the CUs in equal parts: a workgroup
+// ends one tile, takes some whole and begins another. What it has of a tile that others share goes to scratch in float32
+// (256 KB for heads of 256, a dozen sub-blocks' time), and paged_join_tiles_kernel puts it together.
 namespace {
 
 constexpr int PT_ROWS = 64, PT_TILE = 4 * PT_ROWS;
-constexpr int PT_ITEMS = 3;  // items per CU at most when tiles are cut
-constexpr int PT_CUTS = 8;
-
+constexpr int PT_FEW = 3;    // tiles per CU: with as many they go whole, a workgroup each
+constexpr int PT_LEAST = 16;  // sub-blocks of a part
+constexpr int PT_PER_CU(int head_dim) { return head_dim > 64 ? 1 : 2; }  // workgroups that a CU holds
 __device__ __forceinline__ v8bf16 paged_frag(uint32_t at) {
     return *(const __attribute__((address_space(3))) v8bf16*)(uintptr_t)at;
 }
 
-// The tiles of the call, and into how many parts each is cut.
-struct PagedTiles {
-    int jobs, cuts;  // (row, tile, KV head)s; parts of each
+// The sub-blocks [lo, hi) that a tile's query rows see.
+struct PagedSpan {
+    int lo, hi;
 };
 
-__device__ __forceinline__ int paged_row_tiles(const PagedAttnArgs& a, int row, int G) {
-    const PagedRow r = paged_row(a.r, row, a.c.page_size);
+__device__ __forceinline__ PagedSpan paged_span(const PagedAttnArgs& a, const PagedRow& r, int prefix, int tile, int G) {
+    const int first = tile * PT_TILE, lo = paged_sight(a, r, prefix, first / G).lo / 32;
+    return {lo, r.skip ? lo : (paged_sight(a, r, prefix, min((first + PT_TILE - 1) / G, r.n - 1)).hi + 31) / 32};
+}
+
+__device__ __forceinline__ int paged_row_tiles(const PagedAttnArgs& a, const PagedRow& r, int G) {
     return r.n <= 0 || (a.plan.items && r.n * G <= a.plan.few) ? 0 : (r.n * G + PT_TILE - 1) / PT_TILE;
 }
 
-// Parts that end the last item first when every CU takes items of the longest tile's length / parts, each with about 16
-// sub-blocks' time of its own (queries, first loads, sums).
-__device__ __forceinline__ PagedTiles paged_cut(const PagedAttnArgs& a, int G) {
-    int jobs = 0, longest = 0;
-    for (int row = threadIdx.x & 63; row < a.r.rows; row += 64) {
-        const int n = paged_row_tiles(a, row, G);
-        const PagedRow r = paged_row(a.r, row, a.c.page_size);
-        jobs += n;
-        if (n && !r.skip) longest = max(longest, a.window ? min(r.p0 + r.n, a.window + PT_TILE / G + 64) : r.p0 + r.n);
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) jobs += __shfl_xor(jobs, o), longest = max(longest, __shfl_xor(longest, o));
-    jobs *= a.c.kv_heads;
-    longest = (longest + 31) / 32;
-    int cuts = 1, best = 0x7fffffff;
-    for (int c = 1; c <= PT_CUTS && (c == 1 || (jobs * c <= a.plan.cut_slots && longest >= 16 * c)); ++c) {
-        const int cost = ((jobs * c + a.plan.cus - 1) / a.plan.cus) * ((longest + c - 1) / c + 16);
-        if (cost < best) best = cost, cuts = c;
-    }
-    return {__builtin_amdgcn_readfirstlane(jobs), __builtin_amdgcn_readfirstlane(cuts)};
-}
-
-// Job j of the call's: its row, its tile in the row (the latest tokens first) and KV head (fastest: the items of one go to
-// the same XCDs, whose L2 then holds its pages).
-struct PagedJob {
-    int row, tile, kvh;
+// The call's work: `total` units, sub-blocks of its tiles in order (row, tile, KV head) or, `whole`, tiles; in equal `parts`, one
+// per workgroup.
+struct PagedWork {
+    long long total;
+    int jobs, parts;
+    bool whole;
+    __device__ __forceinline__ long long start(int w) const { return total * w / parts; }
+    __device__ __forceinline__ int part(long long u) const { return (int)(((u + 1) * parts - 1) / total); }  // that unit u is in
 };
 
-__device__ __forceinline__ PagedJob paged_job(const PagedAttnArgs& a, int j, int G) {
-    const int lane = threadIdx.x & 63, kvh = j % a.c.kv_heads;
-    int left = j / a.c.kv_heads;
+// The tile that unit u of the call's work is in, and its first unit.
+struct PagedJob {
+    int row, tile, kvh, index;
+    long long start;
+    int units;
+};
+
+__device__ __forceinline__ long long uniform(long long x) {
+    return (long long)uniform((int)(x >> 32)) << 32 | (uint32_t)uniform((int)x);
+}
+
+// Goes over the tiles, a lane for each: 64 rows' numbers of tiles at a time, then 64 of their tiles, whose rows the lanes look up among
+// them. Without `find` it returns the work's total of sub-blocks per KV head, number of tiles and longest tile in job.start, index and units; with it
+// the job of unit u.
+__device__ __forceinline__ PagedJob paged_tiles_list(const PagedAttnArgs& a, int G, bool find, long long u, bool whole) {
+    const int lane = threadIdx.x & 63, Hkv = a.c.kv_heads;
+    long long before = 0;
+    int index = 0, longest = 1;
     for (int base = 0; base < a.r.rows; base += 64) {
-        const int n = base + lane < a.r.rows ? paged_row_tiles(a, base + lane, G) : 0;
+        const int at = min(base + lane, a.r.rows - 1);
+        PagedRow r = paged_row(a.r, at, a.c.page_size);
+        const int prefix = a.prefix ? a.prefix[at] : 0, n = base + lane < a.r.rows ? paged_row_tiles(a, r, G) : 0;
         int ends = n;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const int x = __shfl_up(ends, o);
             if (lane >= o) ends += x;
         }
-        const unsigned long long past = __ballot(ends > left);
-        if (past) {
-            const int l = __ffsll(past) - 1;
-            return {uniform(base + l), uniform(__shfl(ends, l) - 1 - left), kvh};
+        const int count = uniform(__shfl(ends, 63));
+        for (int k0 = 0; k0 < count; k0 += 64) {
+            const int k = k0 + lane;
+            int l = 0;  // the first lane whose rows' tiles end past k
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1)
+                if (__shfl(ends, l + o - 1) <= k) l += o;
+            l = min(l, 63);
+            PagedRow mine;
+            mine.n = __shfl(r.n, l);
+            mine.p0 = __shfl(r.p0, l);
+            mine.skip = __shfl((int)r.skip, l) != 0;
+            mine.t0 = 0;
+            const int tile = __shfl(ends, l) - 1 - k;  // the latest tokens, the longest tiles, first
+            const PagedSpan s = paged_span(a, mine, __shfl(prefix, l), max(tile, 0), G);
+            const int units = k >= count ? 0 : whole ? 1 : max(1, s.hi - s.lo);
+            longest = max(longest, units);
+            long long sum = units;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const long long x = __shfl_up(sum, o);
+                if (lane >= o) sum += x;
+            }
+            const unsigned long long past = find ? __ballot(before + sum * Hkv > u) : 0;
+            if (past) {
+                const int f = __ffsll(past) - 1;
+                PagedJob job;
+                job.row = base + uniform(__shfl(l, f));
+                job.tile = uniform(__shfl(tile, f));
+                job.units = uniform(__shfl(units, f));
+                const long long first = before + uniform(__shfl(sum - units, f)) * Hkv;
+                job.kvh = (int)((u - first) / job.units);
+                job.start = first + (long long)job.kvh * job.units;
+                job.index = (index + k0 + f) * Hkv + job.kvh;
+                return job;
+            }
+            before += uniform(__shfl(sum, 63)) * (find ? Hkv : 1);
         }
-        left -= __shfl(ends, 63);
+        index += count;
     }
-    return {-1, 0, 0};
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) longest = max(longest, __shfl_xor(longest, o));
+    return {-1, 0, 0, index, before, uniform(longest)};
 }
+
+__device__ __forceinline__ PagedWork paged_work(const PagedAttnArgs& a, int G) {
+    const PagedJob all = paged_tiles_list(a, G, false, 0, false);
+    const int jobs = all.index * a.c.kv_heads;
+    const long long total = all.start * a.c.kv_heads;
+    if (!a.plan.parts || jobs >= PT_FEW * a.plan.cus || all.units <= 2 * PT_LEAST) return {jobs, jobs, jobs, true};
+    return {total, jobs, (int)max(1LL, min((long long)a.plan.parts, total / PT_LEAST)), false};
+}
+
+// A cut tile in the scratch's table: which workgroups' sums make it.
+struct PagedCut {
+    int row, tile, kvh, slot, first, last;  // slot: where the first one's are; a later workgroup w's are in slot 2 w
+};
 
 }  // namespace
 
 template <int HD>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void paged_tiles_kernel(const PagedAttnArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PT_PER_CU(HD), PT_PER_CU(HD)))) void paged_tiles_kernel(const PagedAttnArgs a) {
     constexpr int TILE = 32;                   // positions per LDS buffer
     constexpr int NI = HD > 128 ? 2 : 1;       // 16-byte pieces of keys, and of values, per thread (heads of 64: of either)
     constexpr bool EITHER = HD == 64;
@@ -494,21 +547,33 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     __shared__ int lost[3][2];
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, h = lane >> 5;
     const int Hkv = a.c.kv_heads, G = a.q_heads / Hkv, ps = a.c.page_size, shift = __builtin_ctz(ps);
-    const PagedTiles all = paged_cut(a, G);
-    const int z = blockIdx.x / max(all.jobs, 1), j = blockIdx.x % max(all.jobs, 1);
-    if (z >= all.cuts || !all.jobs) return;
-    const PagedJob job = paged_job(a, j, G);
+    const PagedWork work = paged_work(a, G);
+    if (blockIdx.x == 0 && threadIdx.x == 0 && a.plan.parts) *(int*)(a.scratch + a.plan.cuts) = work.whole ? 0 : work.jobs;
+    const int w = blockIdx.x;
+    if (!work.jobs || w >= work.parts) return;
+    const long long begin = work.start(w), end = work.start(w + 1);
+    for (long long unit = begin; unit < end;) {
+    const PagedJob job = paged_tiles_list(a, G, true, unit, work.whole);
     if (job.row < 0) return;
     const PagedRow r = paged_row_uniform(a.r, job.row, ps);
     const int R = r.n * G, total = r.p0 + r.n, prefix = a.prefix ? uniform(a.prefix[job.row]) : 0;
-    const int first = job.tile * PT_TILE, i_last = min((first + PT_TILE - 1) / G, r.n - 1);  // the tile's first query row, its last token
+    const int first = job.tile * PT_TILE;  // the tile's first query row
     const int* table = a.r.pages + (size_t)job.row * a.r.max_pages;
-
-    // The tiles of positions that any of the workgroup's rows sees; this item's.
-    const int lo_tile = paged_sight(a, r, prefix, first / G).lo / TILE, hi_tile = r.skip ? lo_tile : (paged_sight(a, r, prefix, i_last).hi + TILE - 1) / TILE;
-    const int T0 = lo_tile + (int)((long long)(hi_tile - lo_tile) * z / all.cuts), T1 = lo_tile + (int)((long long)(hi_tile - lo_tile) * (z + 1) / all.cuts);
+    // This part's tiles of positions of those that any of the workgroup's query rows sees.
+    const PagedSpan span = paged_span(a, r, prefix, job.tile, G);
+    const long long stop = min(end, job.start + job.units);
+    const int T0 = span.lo + (work.whole ? 0 : (int)(unit - job.start)), T1 = work.whole ? span.hi : min(span.hi, span.lo + (int)(stop - job.start));
+    const bool alone = unit == job.start && stop == job.start + job.units;
+    const int slot = 2 * w + (unit > begin);
+    if (unit == job.start && !work.whole && threadIdx.x == 0)
+        ((PagedCut*)(a.scratch + a.plan.cuts + 256))[job.index] = {job.row, job.tile, job.kvh, slot, w, alone ? w : work.part(job.start + job.units - 1)};
+    unit = stop;
 
     const int row0 = first + wv * PT_ROWS;
+    // The queries as B operands, in registers but for the last QS of a lane's second row, which wait in LDS: with them the loop
+    // would reload others from scratch memory, each time behind every load under way.
+    constexpr int QS = HD > 128 ? 8 : 0;
+    __shared__ __attribute__((aligned(16))) v8bf16 q_last[QS ? QS * 256 : 1];
     v8bf16 qf[2][KM];
     int token[2];  // of this lane's query rows; -1: none
     __shared__ float slopes[PT_TILE];
@@ -521,8 +586,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
         const bf16_t* qp = a.q + ((size_t)(r.t0 + (mine ? i : 0)) * a.q_heads + (mine ? head : 0)) * HD + h * 8;
 #pragma unroll
         for (int m = 0; m < KM; ++m) {
-            qf[rt][m] = *(const v8bf16*)(qp + m * 16);
-            if (!mine) qf[rt][m] = (v8bf16)(__bf16)0.0f;
+            v8bf16 x = *(const v8bf16*)(qp + m * 16);
+            if (!mine) x = (v8bf16)(__bf16)0.0f;
+            if (rt && m >= KM - QS)
+                q_last[(m - (KM - QS)) * 256 + threadIdx.x] = x;
+            else
+                qf[rt][m] = x;
         }
     }
     const PagedSight early = paged_sight(a, r, prefix, min(row0, R - 1) / G), late = paged_sight(a, r, prefix, min(row0 + PT_ROWS - 1, R - 1) / G);
@@ -611,28 +680,28 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     float top[2] = {UNSEEN, UNSEEN}, most[2] = {-INFINITY, -INFINITY}, sum[2];
 
     // Scores of sub-block n, with the loaded tile (n + 1) widened beside their MFMAs; then what the weights are relative to.
-    auto scores = [&](int n, auto more) __attribute__((always_inline)) {
+    auto scores = [&](int n) __attribute__((always_inline)) {
         const uint32_t ka = lds0 + n % 3 * BUF + kl;
-        v8bf16 kf[DEEP];
+        v8bf16 kf[DEEP], qx[2];
 #pragma unroll
         for (int m = 0; m < DEEP; ++m) kf[m] = paged_frag(ka ^ (m << 5));
 #pragma unroll
         for (int m = 0; m < KM; ++m) {
             __builtin_amdgcn_sched_barrier(0);
+            const v8bf16 q1 = m < KM - QS ? qf[1][m] : qx[m & 1];
             if (m)
                 asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %2, %3, %0\n\tv_mfma_f32_32x32x16_bf16 %1, %2, %4, %1"
-                             : "+v"(s[0]), "+v"(s[1]) : "v"(kf[m % DEEP]), "v"(qf[0][m]), "v"(qf[1][m]));
+                             : "+v"(s[0]), "+v"(s[1]) : "v"(kf[m % DEEP]), "v"(qf[0][m]), "v"(q1));
             else
                 asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %2, %3, 0\n\tv_mfma_f32_32x32x16_bf16 %1, %2, %4, 0"
-                             : "=&v"(s[0]), "=&v"(s[1]) : "v"(kf[m % DEEP]), "v"(qf[0][m]), "v"(qf[1][m]));
+                             : "=&v"(s[0]), "=&v"(s[1]) : "v"(kf[m % DEEP]), "v"(qf[0][m]), "v"(q1));
+            if (m + 2 < KM && m + 2 >= KM - QS) qx[m & 1] = q_last[(m + 2 - (KM - QS)) * 256 + threadIdx.x];
             if (m + DEEP < KM) kf[m % DEEP] = paged_frag(ka ^ ((m + DEEP) << 5));
-            if constexpr (decltype(more)::value)
-                if (m >= KM - STEPS) widen(n + 1, m - (KM - STEPS));
+            if (m >= KM - STEPS) widen(n + 1, m - (KM - STEPS));
         }
-        if constexpr (decltype(more)::value) {  // as early as the registers are free again: a tile's time before they are widened
-            load(min(n + 2, T1 - 1));
-            look(min(n + 3, T1 - 1));
-        }
+        // As early as the registers are free again: a tile's time before they are widened.
+        load(min(n + 2, T1 - 1));
+        look(min(n + 3, T1 - 1));
         __builtin_amdgcn_sched_barrier(0);
         asm volatile("s_nop 15\n\ts_nop 15" : "+v"(s[0]), "+v"(s[1]));  // the last products' way into the registers
         const int p0 = n * 32;
@@ -735,20 +804,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
         for (int x = 0; x < STEPS; ++x) widen(T0, x);
         load(min(T0 + 1, T1 - 1));
         look(min(T0 + 2, T1 - 1));
-#pragma unroll
-        for (int x = 0; x < STEPS; ++x) widen(T0 + 1, x);
-        load(min(T0 + 2, T1 - 1));
-        look(min(T0 + 3, T1 - 1));
-        __syncthreads();
         // Tile T is in buffer T % 3. A tile is widened into the buffer of the one three before, whose last weights x V every
         // wave has behind it when it comes to the barrier that a tile begins with.
-        scores(T0, std::false_type{});
-#pragma unroll
-        for (int x = 0; x < 16; ++x) weight2(x, pw);
-        for (int T = T0; T + 1 < T1; ++T) {
+        for (int T = T0; T < T1; ++T) {
             __syncthreads();
-            scores(T + 1, std::true_type{});
-            values(T, std::true_type{});
+            scores(T);
+            if (T > T0)
+                values(T - 1, std::true_type{});
+            else
+#pragma unroll
+                for (int x = 0; x < 16; ++x) weight2(x, pw);
         }
         values(T1 - 1, std::false_type{});
         bool leapt = false;
@@ -762,7 +827,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
         for (int rt = 0; rt < 2; ++rt) top[rt] = fmaxf(top[rt], most[rt]);
     }
 
-    if (all.cuts == 1) {
+    if (alone) {
 #pragma unroll
         for (int rt = 0; rt < 2; ++rt) {
             const float l = sum[rt] + __shfl_xor(sum[rt], 32), inv = r.skip ? 0.0f : 1.0f / l;
@@ -776,10 +841,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
                     *(uint2*)(out + d * 32 + q * 8) = make_uint2(pk_bf16(o[rt][d][4 * q] * inv, o[rt][d][4 * q + 1] * inv),
                                                                  pk_bf16(o[rt][d][4 * q + 2] * inv, o[rt][d][4 * q + 3] * inv));
         }
-        return;
-    }
-    // [item][wave][rt][d][q][lane] of four dims, then per query row its maximum and sum.
-    float* part = (float*)(a.scratch + a.plan.cut_part) + (size_t)(j * all.cuts + z) * (PT_TILE * (HD + 2));
+    } else {
+    // [slot][wave][rt][d][q][lane] of four dims, then per query row its maximum and sum.
+    float* part = (float*)(a.scratch + a.plan.cut_part) + (size_t)slot * (PT_TILE * (HD + 2));
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {
         const float l = sum[rt] + __shfl_xor(sum[rt], 32);
@@ -790,34 +854,36 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
             for (int q = 0; q < 4; ++q)
                 *(v4f*)(part + ((((wv * 2 + rt) * VD + d) * 4 + q) * 64 + lane) * 4) = (v4f){o[rt][d][4 * q], o[rt][d][4 * q + 1], o[rt][d][4 * q + 2], o[rt][d][4 * q + 3]};
     }
+    }
+    __syncthreads();  // the ring and the slopes are the next tile's
+    }
 }
 
-// The parts of cut tiles put together. Grid: jobs x the tile's eight groups of 32 query rows x dims in blocks of 32.
+// The parts of cut tiles put together. Grid: tiles x the tile's eight groups of 32 query rows x dims in blocks of 32.
 template <int HD>
 __global__ __launch_bounds__(256) void paged_join_tiles_kernel(const PagedAttnArgs a) {
     constexpr int VD = HD / 32;
     const int lane = threadIdx.x & 63, q = threadIdx.x >> 6, l32 = lane & 31, h = lane >> 5;
     const int Hkv = a.c.kv_heads, G = a.q_heads / Hkv;
-    const PagedTiles all = paged_cut(a, G);
     const int d = blockIdx.x % VD, group = blockIdx.x / VD % 8, j = blockIdx.x / VD / 8;
-    if (all.cuts == 1 || j >= all.jobs) return;
-    const PagedJob job = paged_job(a, j, G);
-    if (job.row < 0) return;
+    if (j >= *(const int*)(a.scratch + a.plan.cuts)) return;
+    const PagedCut job = ((const PagedCut*)(a.scratch + a.plan.cuts + 256))[j];
+    if (job.first == job.last) return;
     const PagedRow r = paged_row(a.r, job.row, a.c.page_size);
     const int row = job.tile * PT_TILE + group * 32 + l32;
     if (row >= r.n * G) return;
     const size_t step = PT_TILE * (HD + 2);
-    const float* part = (const float*)(a.scratch + a.plan.cut_part) + (size_t)j * all.cuts * step;
-    const float* stats = part + PT_TILE * HD + (group * 32 + l32) * 2;
+    const float* part = (const float*)(a.scratch + a.plan.cut_part);
+    const size_t stats = PT_TILE * HD + (group * 32 + l32) * 2, dims = ((((size_t)group * VD + d) * 4 + q) * 64 + lane) * 4;
+    auto slot = [&](int w) { return (w == job.first ? job.slot : 2 * w) * step; };
     float top = -INFINITY, l = 0.0f;
-    for (int z = 0; z < all.cuts; ++z) top = fmaxf(top, stats[z * step]);
+    for (int w = job.first; w <= job.last; ++w) top = fmaxf(top, part[slot(w) + stats]);
     v4f o = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
-    for (int z = 0; z < all.cuts; ++z) {
-        const float2 s = *(const float2*)(stats + z * step);
+    for (int w = job.first; w <= job.last; ++w) {
+        const float2 s = *(const float2*)(part + slot(w) + stats);
         const float f = s.x == top ? 1.0f : exp2_(s.x - top);  // the same where no part saw anything, or only NaN
         l += s.y * f;
-        const v4f v = *(const v4f*)(part + z * step + ((((size_t)group * VD + d) * 4 + q) * 64 + lane) * 4);
-        o += v * f;
+        o += *(const v4f*)(part + slot(w) + dims) * f;
     }
     const float inv = r.skip ? 0.0f : 1.0f / l;
     *(uint2*)(a.out + ((size_t)(r.t0 + row / G) * a.q_heads + job.kvh * G + row % G) * HD + d * 32 + q * 8 + h * 4) =
@@ -844,14 +910,16 @@ PagedPlan paged_attention_plan(const PagedCache& c, const PagedRows& r, int q_he
     if (most > p.few) {
         const long long jobs = heads * ((most + PT_TILE - 1) / PT_TILE);
         p.cus = q38_device_cus();
-        // Tiles are cut only while that gives at most PT_ITEMS items per CU, so at most half as many tiles are.
-        const long long longest = (long long)r.max_pages * c.page_size + r.max_tokens;
-        const bool cut = longest >= 2 * 16 * 32 && (r.q_start || jobs * 2 <= PT_ITEMS * p.cus);
-        p.cut_slots = cut ? (int)std::min<long long>(PT_ITEMS * p.cus, jobs * PT_CUTS) : 0;
-        p.cut_jobs = std::min<long long>(p.cut_slots / 2, jobs);
-        p.tiles = (int)std::max<long long>(jobs, p.cut_slots);
-        p.cut_part = p.bytes + 255 & ~(size_t)255;
-        p.bytes = p.cut_part + (size_t)p.cut_slots * PT_TILE * (c.head_dim + 2) * 4;
+        const long long blocks = ((long long)r.max_pages * c.page_size + r.max_tokens + 31) / 32 + 1;
+        const bool many = jobs >= (long long)PT_FEW * p.cus;
+        p.parts = many && !r.q_start ? 0 : (int)std::min<long long>(p.cus * PT_PER_CU(c.head_dim), std::max<long long>(1, jobs * blocks / PT_LEAST));
+        p.tiles = (int)std::max<long long>(p.parts, jobs);
+        if (p.parts) {
+            p.cut_jobs = (int)std::min<long long>(jobs, (long long)PT_FEW * p.cus);
+            p.cuts = p.bytes + 255 & ~(size_t)255;
+            p.cut_part = p.cuts + 256 + (size_t)p.cut_jobs * sizeof(PagedCut) + 255 & ~(size_t)255;
+            p.bytes = p.cut_part + (size_t)2 * p.parts * PT_TILE * (c.head_dim + 2) * 4;
+        }
     }
     return p;
 }
@@ -885,7 +953,7 @@ hipError_t q38_paged_attention(const PagedAttnArgs& a, hipStream_t stream) {
 #define TILES(HD)                                                                                                             \
     do {                                                                                                                     \
         hipLaunchKernelGGL((paged_tiles_kernel<HD>), dim3(a.plan.tiles), dim3(256), 0, stream, a);                           \
-        if (a.plan.cut_slots) hipLaunchKernelGGL((paged_join_tiles_kernel<HD>), dim3(a.plan.cut_jobs * 8 * (HD / 32)), dim3(256), 0, stream, a); \
+        if (a.plan.parts) hipLaunchKernelGGL((paged_join_tiles_kernel<HD>), dim3(a.plan.cut_jobs * 8 * (HD / 32)), dim3(256), 0, stream, a); \
     } while (0)
     switch (a.c.head_dim) {
         case 64: TILES(64); break;
