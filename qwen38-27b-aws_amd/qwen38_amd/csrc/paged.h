@@ -76,9 +76,8 @@ __device__ __forceinline__ PagedRow paged_row(const PagedRows& a, int row, int p
 
 // The page that holds position p of the row whose table entries are at `table`, or -1.
 __device__ __forceinline__ int paged_find(const PagedRows& a, const int* table, int page, int pages) {
-    if (page < 0 || page >= a.max_pages) return -1;
-    const int id = table[page];
-    return id >= 0 && id < pages ? id : -1;
+    const int id = table[min(max(page, 0), a.max_pages - 1)];  // read in any case: a choice, not a branch
+    return ((page >= 0) & (page < a.max_pages) & (id >= 0) & (id < pages)) ? id : -1;
 }
 
 hipError_t q38_paged_append(const PagedAppendArgs& a, hipStream_t stream);

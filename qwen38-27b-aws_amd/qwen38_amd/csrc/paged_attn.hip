@@ -47,6 +47,15 @@ __device__ __forceinline__ v8bf16 paged_widen(uint32_t w0, uint32_t w1, float sc
     return __builtin_bit_cast(v8bf16, r);
 }
 
+typedef __bf16 v4bf16 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ v4bf16 paged_widen2(uint32_t w, float scale) {
+    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+    const u2 r = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false)),
+                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true))};
+    return __builtin_bit_cast(v4bf16, r);
+}
+
 __device__ __forceinline__ float paged_scale(int byte) { return __uint_as_float((uint32_t)byte << 23); }
 
 // Scores to powers of two: capped and biased as the call asks.
@@ -570,10 +579,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PT_PER_CU(H
     unit = stop;
 
     const int row0 = first + wv * PT_ROWS;
-    // The queries as B operands, in registers but for the last QS of a lane's second row, which wait in LDS: with them the loop
+    // The queries as B operands, in registers but for the first QS of a lane's second row, which wait in LDS: with them the loop
     // would reload others from scratch memory, each time behind every load under way.
-    constexpr int QS = HD > 128 ? 8 : 0;
-    __shared__ __attribute__((aligned(16))) v8bf16 q_last[QS ? QS * 256 : 1];
+    constexpr int QS = HD > 128 ? 10 : 0;
+    __shared__ __attribute__((aligned(16))) v8bf16 q_wait[QS ? QS * 256 : 1];
     v8bf16 qf[2][KM];
     int token[2];  // of this lane's query rows; -1: none
     __shared__ float slopes[PT_TILE];
@@ -588,8 +597,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PT_PER_CU(H
         for (int m = 0; m < KM; ++m) {
             v8bf16 x = *(const v8bf16*)(qp + m * 16);
             if (!mine) x = (v8bf16)(__bf16)0.0f;
-            if (rt && m >= KM - QS)
-                q_last[(m - (KM - QS)) * 256 + threadIdx.x] = x;
+            if (rt && m < QS)
+                q_wait[m * 256 + threadIdx.x] = x;
             else
                 qf[rt][m] = x;
         }
@@ -605,15 +614,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PT_PER_CU(H
     auto look = [&](int T) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            const int page = (T * TILE + (vg0 + i) * 16) >> shift;
-            found[i] = page < a.r.max_pages ? table[page] : -1;
+            found[i] = table[min((T * TILE + (vg0 + i) * 16) >> shift, a.r.max_pages - 1)];
         }
     };
-    auto load = [&](int T) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < NI; ++i) {
+    auto load = [&](int T, int i) __attribute__((always_inline)) {
+        {
             id[i] = uniform(found[i]);
-            id[i] = id[i] < a.c.pages ? id[i] : -1;
+            id[i] = ((id[i] < a.c.pages) & ((T * TILE + (vg0 + i) * 16) >> shift < a.r.max_pages)) ? id[i] : -1;
             const size_t head = (size_t)max(id[i], 0) * Hkv + job.kvh, at = (head * ps + ((T * TILE + (vg0 + i) * 16) & (ps - 1))) * HD;
             if constexpr (EITHER) {
                 ks[i] = (wv < 2 ? a.c.k_scale : a.c.v_scale)[head];
@@ -626,17 +633,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PT_PER_CU(H
             }
         }
     };
-    // Step x of widening the loaded tile T into its buffer: half of a piece. Keys: row (position), its 16-byte chunks spread
+    // Step x of widening the loaded tile T into its buffer, or half of that: half of a piece. Keys: row (position), its 16-byte chunks spread
     // over the banks; values: per dim 32 positions, likewise.
     const uint32_t lds0 = (uint32_t)(uintptr_t)LDS_PTR(&ring[0]);
     const int kp0 = c0 / (HD / 16), kc0 = c0 % (HD / 16) * 2, vd0 = c0 % HD;
     const uint32_t put_k = kp0 * HD * 2 + ((kc0 ^ (HD > 64 ? kp0 & 15 : (kp0 >> 1) & 7)) << 4);
     const uint32_t put_v = HALF + vd0 * 64 + ((vg0 * 2 ^ ((vd0 >> 1) & 3) ^ ((vd0 >> 3) & 1)) << 4);
     auto put = [&](uint32_t at, v8bf16 x) __attribute__((always_inline)) { *(__attribute__((address_space(3))) v8bf16*)(uintptr_t)at = x; };
-    auto widen = [&](int T, int x) __attribute__((always_inline)) {
+    v8bf16 piece;
+    auto widen = [&](int T, int x, int half = -1) __attribute__((always_inline)) {
         const uint32_t buf = lds0 + T % 3 * BUF;
         const int i = EITHER ? 0 : x >> 2, u = x & 1;
-        if (x == 0) {
+        if (x == 0 && half < 1) {
             // Bytes that no token wrote may be anything, and so may those of a page that is not there.
             bool tail = T * TILE + TILE > total;
 #pragma unroll
@@ -655,12 +663,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PT_PER_CU(H
             for (int k = 0; k < NI; ++k)
                 if (vd0 == 0) lost[T % 3][vg0 + k] = id[k] < 0;
         }
-        if (EITHER ? wv < 2 : !(x & 2))
-            put(buf + i * (256 / (HD / 16) * HD * 2) + (put_k ^ (u << 4)), u ? paged_widen(rk[i].z, rk[i].w, paged_scale(ks[i])) : paged_widen(rk[i].x, rk[i].y, paged_scale(ks[i])));
-        else if constexpr (EITHER)
-            put(buf + (put_v ^ (u << 4)), u ? paged_widen(rk[0].z, rk[0].w, paged_scale(ks[0])) : paged_widen(rk[0].x, rk[0].y, paged_scale(ks[0])));
-        else
-            put(buf + (put_v ^ (i << 5) ^ (u << 4)), u ? paged_widen(rv[i].z, rv[i].w, paged_scale(vs[i])) : paged_widen(rv[i].x, rv[i].y, paged_scale(vs[i])));
+        const bool key = EITHER ? wv < 2 : !(x & 2);
+        const uint4 w = EITHER || key ? rk[i] : rv[i];
+        const float scale = paged_scale(EITHER || key ? ks[i] : vs[i]);
+        if (half < 1) piece = __builtin_shufflevector(paged_widen2(u ? w.z : w.x, scale), paged_widen2(u ? w.z : w.x, scale), 0, 1, 2, 3, -1, -1, -1, -1);
+        if (half != 0) {
+            const v4bf16 last = paged_widen2(u ? w.w : w.y, scale);
+            const uint32_t at = key ? i * (256 / (HD / 16) * HD * 2) + (put_k ^ (u << 4)) : put_v ^ (i << 5) ^ (u << 4);
+            put(buf + at, __builtin_shufflevector(__builtin_shufflevector(piece, piece, 0, 1, 2, 3), last, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
     };
 
     const int kp = (l32 & ~12) | (l32 & 4) << 1 | (l32 & 8) >> 1;  // the position of this lane's key row
@@ -679,33 +690,45 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PT_PER_CU(H
     constexpr float LEAP = 40.0f, UNSEEN = -3e38f;
     float top[2] = {UNSEEN, UNSEEN}, most[2] = {-INFINITY, -INFINITY}, sum[2];
 
+    bool unseen = true;  // some row's reference is not known yet
+    // The largest of three, NaN ones passed over.
+    auto max3 = [](float x, float y, float z) __attribute__((always_inline)) {
+        float m;
+        asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(x), "v"(y), "v"(z));
+        return m;
+    };
     // Scores of sub-block n, with the loaded tile (n + 1) widened beside their MFMAs; then what the weights are relative to.
     auto scores = [&](int n) __attribute__((always_inline)) {
         const uint32_t ka = lds0 + n % 3 * BUF + kl;
+        const int gone0 = lost[n % 3][0], gone1 = lost[n % 3][1];
         v8bf16 kf[DEEP], qx[2];
 #pragma unroll
         for (int m = 0; m < DEEP; ++m) kf[m] = paged_frag(ka ^ (m << 5));
 #pragma unroll
+        for (int m = 0; m < 2 && m < QS; ++m) qx[m] = q_wait[m * 256 + threadIdx.x];
+#pragma unroll
         for (int m = 0; m < KM; ++m) {
+            const v8bf16 q1 = m < QS ? qx[m & 1] : qf[1][m];
             __builtin_amdgcn_sched_barrier(0);
-            const v8bf16 q1 = m < KM - QS ? qf[1][m] : qx[m & 1];
             if (m)
-                asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %2, %3, %0\n\tv_mfma_f32_32x32x16_bf16 %1, %2, %4, %1"
-                             : "+v"(s[0]), "+v"(s[1]) : "v"(kf[m % DEEP]), "v"(qf[0][m]), "v"(q1));
+                asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(s[0]) : "v"(kf[m % DEEP]), "v"(qf[0][m]));
             else
-                asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %2, %3, 0\n\tv_mfma_f32_32x32x16_bf16 %1, %2, %4, 0"
-                             : "=&v"(s[0]), "=&v"(s[1]) : "v"(kf[m % DEEP]), "v"(qf[0][m]), "v"(q1));
-            if (m + 2 < KM && m + 2 >= KM - QS) qx[m & 1] = q_last[(m + 2 - (KM - QS)) * 256 + threadIdx.x];
+                asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(s[0]) : "v"(kf[m % DEEP]), "v"(qf[0][m]));
+            const int x = m - (KM - STEPS);
+            if (x >= 0) widen(n + 1, x, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            if (m)
+                asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(s[1]) : "v"(kf[m % DEEP]), "v"(q1));
+            else
+                asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(s[1]) : "v"(kf[m % DEEP]), "v"(q1));
+            if (m + 2 < QS) qx[m & 1] = q_wait[(m + 2) * 256 + threadIdx.x];
             if (m + DEEP < KM) kf[m % DEEP] = paged_frag(ka ^ ((m + DEEP) << 5));
-            if (m >= KM - STEPS) widen(n + 1, m - (KM - STEPS));
+            if (x >= 0) widen(n + 1, x, 1);
         }
-        // As early as the registers are free again: a tile's time before they are widened.
-        load(min(n + 2, T1 - 1));
-        look(min(n + 3, T1 - 1));
         __builtin_amdgcn_sched_barrier(0);
         asm volatile("s_nop 15\n\ts_nop 15" : "+v"(s[0]), "+v"(s[1]));  // the last products' way into the registers
         const int p0 = n * 32;
-        const int lost0 = uniform(lost[n % 3][0]), lost1 = uniform(lost[n % 3][1]);
+        const int lost0 = uniform(gone0), lost1 = uniform(gone1);
         if (bent) {
 #pragma unroll
             for (int rt = 0; rt < 2; ++rt)
@@ -732,35 +755,35 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PT_PER_CU(H
                 }
             }
         }
-        // Of seen scores; NaN ones are passed over.
-        auto max3 = [](float x, float y, float z) __attribute__((always_inline)) {
-            float m;
-            asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(x), "v"(y), "v"(z));
-            return m;
-        };
-#pragma unroll
-        for (int rt = 0; rt < 2; ++rt)
-#pragma unroll
-            for (int e = 0; e < 16; e += 2) most[rt] = max3(s[rt][e], s[rt][e + 1], most[rt]);
-        if (__any((top[0] == UNSEEN) | (top[1] == UNSEEN))) {
+        if (unseen) {
 #pragma unroll
             for (int rt = 0; rt < 2; ++rt) {
-                const float m = fmaxf(most[rt], __shfl_xor(most[rt], 32)) * mul;
+                float m = -INFINITY;
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) m = max3(s[rt][e], s[rt][e + 1], m);
+                m = fmaxf(m, __shfl_xor(m, 32)) * mul;
                 top[rt] = ((top[rt] == UNSEEN) & (m > -INFINITY)) ? m : top[rt];
             }
+            unseen = __any((top[0] == UNSEEN) | (top[1] == UNSEEN));
         }
     };
-    auto weight2 = [&](int x, u4_ (&w)[2][2]) __attribute__((always_inline)) {
-        const int rt = x >> 3, e = 2 * (x & 7);
-        const float e0 = exp2_(__builtin_fmaf(s[rt][e], mul, -top[rt])), e1 = exp2_(__builtin_fmaf(s[rt][e + 1], mul, -top[rt]));
-        sum[rt] += e0;
-        sum[rt] += e1;
-        uint32_t both = pk_bf16(e0, e1);
-        asm volatile("" : "+v"(both));  // here, beside the MFMAs, not where it is first used
-        w[rt][(x >> 2) & 1][x & 3] = both;
+    // Weight x of the lane's 32.
+    float even;
+    auto weight = [&](int x, u4_ (&w)[2][2]) __attribute__((always_inline)) {
+        const int rt = x >> 4, e = x & 15;
+        const float p = exp2_(__builtin_fmaf(s[rt][e], mul, -top[rt]));
+        sum[rt] += p;
+        if (e & 1) {
+            most[rt] = max3(s[rt][e - 1], s[rt][e], most[rt]);
+            uint32_t both = pk_bf16(even, p);
+            asm volatile("" : "+v"(both));  // here, beside the MFMAs, not where it is first used
+            w[rt][e >> 3][(e >> 1) & 3] = both;
+        }
+        even = p;
     };
     // Weights x V of sub-block n, beside them the next one's weights.
     auto values = [&](int n, auto next) __attribute__((always_inline)) {
+        __builtin_amdgcn_sched_barrier(0);
         const uint32_t va = lds0 + n % 3 * BUF + vl;
         auto frag = [&](int x) __attribute__((always_inline)) { return paged_frag((va ^ ((x & 1) << 5)) + (x >> 1) * 2048); };
         v8bf16 vf[DEEP];
@@ -769,14 +792,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PT_PER_CU(H
         u4_ nw[2][2];
 #pragma unroll
         for (int x = 0; x < 2 * VD; ++x) {
-            __builtin_amdgcn_sched_barrier(0);
+            // A wave's own instructions run beside an MFMA only until the next one: they go between the two of a step as well.
 #pragma unroll
-            for (int rt = 0; rt < 2; ++rt)
+            for (int rt = 0; rt < 2; ++rt) {
+                __builtin_amdgcn_sched_barrier(0);
                 o[rt][x >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[x % DEEP], __builtin_bit_cast(v8bf16, pw[rt][x & 1]), o[rt][x >> 1], 0, 0, 0);
-            if (x + DEEP < 2 * VD) vf[x % DEEP] = frag(x + DEEP);
-            if constexpr (decltype(next)::value)
+                __builtin_amdgcn_sched_barrier(0);
+                if (rt && x + DEEP < 2 * VD) vf[x % DEEP] = frag(x + DEEP);
+                if constexpr (decltype(next)::value) {
+                    if (rt && x < NI) load(min(n + 3, T1 - 1), x);
+                    if (rt && x == NI) look(min(n + 4, T1 - 1));
 #pragma unroll
-                for (int y = 0; y < 8 / VD; ++y) weight2(x * (8 / VD) + y, nw);
+                    for (int y = 0; y < 8 / VD; ++y) weight((2 * x + rt) * (8 / VD) + y, nw);
+                }
+            }
         }
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (decltype(next)::value) {
@@ -797,23 +826,31 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PT_PER_CU(H
                 for (int e = 0; e < 16; ++e) o[rt][d][e] = 0.0f;
         }
         if (T0 >= T1) break;
+        auto load_all = [&](int T) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i) load(T, i);
+        };
         look(T0);
-        load(T0);
+        load_all(T0);
         look(min(T0 + 1, T1 - 1));
 #pragma unroll
         for (int x = 0; x < STEPS; ++x) widen(T0, x);
-        load(min(T0 + 1, T1 - 1));
+        load_all(min(T0 + 1, T1 - 1));
         look(min(T0 + 2, T1 - 1));
         // Tile T is in buffer T % 3. A tile is widened into the buffer of the one three before, whose last weights x V every
-        // wave has behind it when it comes to the barrier that a tile begins with.
+        // wave has behind it when it comes to the barrier that a tile begins with. The tile after it is loaded as soon as its
+        // registers are free: most of a tile's time before it is widened.
         for (int T = T0; T < T1; ++T) {
             __syncthreads();
             scores(T);
-            if (T > T0)
+            if (T > T0) {
                 values(T - 1, std::true_type{});
-            else
+            } else {
 #pragma unroll
-                for (int x = 0; x < 16; ++x) weight2(x, pw);
+                for (int x = 0; x < 32; ++x) weight(x, pw);
+                load_all(min(T0 + 2, T1 - 1));
+                look(min(T0 + 3, T1 - 1));
+            }
         }
         values(T1 - 1, std::false_type{});
         bool leapt = false;
