@@ -424,7 +424,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) 
 // (256 KB for heads of 256, a dozen sub-blocks' time), and paged_join_tiles_kernel puts it together.
 namespace {
 
-constexpr int PT_ROWS = 64, PT_TILE = 4 * PT_ROWS;
+constexpr int PT_TILE = 256;
 constexpr int PT_FEW = 3;    // tiles per CU: with as many they go whole, a workgroup each
 constexpr int PT_LEAST = 16;  // sub-blocks of a part
 constexpr int PT_PER_CU(int head_dim) { return head_dim > 64 ? 1 : 2; }  // workgroups that a CU holds
@@ -545,16 +545,17 @@ struct PagedCut {
 }  // namespace
 
 template <int HD>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PT_PER_CU(HD), PT_PER_CU(HD)))) void paged_tiles_kernel(const PagedAttnArgs a) {
-    constexpr int TILE = 32;                   // positions per LDS buffer
-    constexpr int NI = HD > 128 ? 2 : 1;       // 16-byte pieces of keys, and of values, per thread (heads of 64: of either)
-    constexpr bool EITHER = HD == 64;
-    constexpr int KM = HD / 16, VD = HD / 32, HALF = TILE * HD * 2, BUF = 2 * HALF;  // MFMA steps; bytes of a buffer's keys, of a buffer
-    constexpr int DEEP = HD > 128 ? 3 : 4;     // operands read ahead from LDS
-    constexpr int STEPS = EITHER ? 2 : 4 * NI;  // pieces of widening: 8 bf16 each
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_tiles_kernel(const PagedAttnArgs a) {
+    constexpr int KM = HD / 16, VD = HD / 32, HALF = 32 * HD * 2, BUF = 2 * HALF;  // MFMA steps; bytes of a buffer's keys, of a buffer
+    constexpr int PIECES = 2 * HD;       // 16-byte pieces of a tile's keys, and of its values: one of each per thread, or of either
+    constexpr bool BOTH = HD == 256;
+    constexpr int STEPS = BOTH ? 4 : 2;  // half pieces to widen
+    constexpr int DEEP = HD > 128 ? 2 : 4;  // operands read ahead from LDS
+    constexpr int CHAINS = HD > 128 ? 1 : 2;  // sums that a score is made of
     __shared__ __attribute__((aligned(1024))) uint8_t ring[3 * BUF];
     __shared__ int lost[3][2];
-    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, h = lane >> 5;
+    __shared__ float slopes[PT_TILE];
+    const int lane = threadIdx.x & 63, wv = uniform((int)threadIdx.x >> 6), l32 = lane & 31, h = lane >> 5;
     const int Hkv = a.c.kv_heads, G = a.q_heads / Hkv, ps = a.c.page_size, shift = __builtin_ctz(ps);
     const PagedWork work = paged_work(a, G);
     if (blockIdx.x == 0 && threadIdx.x == 0 && a.plan.parts) *(int*)(a.scratch + a.plan.cuts) = work.whole ? 0 : work.jobs;
@@ -566,9 +567,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PT_PER_CU(H
     if (job.row < 0) return;
     const PagedRow r = paged_row_uniform(a.r, job.row, ps);
     const int R = r.n * G, total = r.p0 + r.n, prefix = a.prefix ? uniform(a.prefix[job.row]) : 0;
-    const int first = job.tile * PT_TILE;  // the tile's first query row
     const int* table = a.r.pages + (size_t)job.row * a.r.max_pages;
-    // This part's tiles of positions of those that any of the workgroup's query rows sees.
+    // This part's tiles of 32 positions of those that any of the workgroup's query rows sees.
     const PagedSpan span = paged_span(a, r, prefix, job.tile, G);
     const long long stop = min(end, job.start + job.units);
     const int T0 = span.lo + (work.whole ? 0 : (int)(unit - job.start)), T1 = work.whole ? span.hi : min(span.hi, span.lo + (int)(stop - job.start));
@@ -578,118 +578,93 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PT_PER_CU(H
         ((PagedCut*)(a.scratch + a.plan.cuts + 256))[job.index] = {job.row, job.tile, job.kvh, slot, w, alone ? w : work.part(job.start + job.units - 1)};
     unit = stop;
 
-    const int row0 = first + wv * PT_ROWS;
-    // The queries as B operands, in registers but for the first QS of a lane's second row, which wait in LDS: with them the loop
-    // would reload others from scratch memory, each time behind every load under way.
-    constexpr int QS = HD > 128 ? 10 : 0;
-    __shared__ __attribute__((aligned(16))) v8bf16 q_wait[QS ? QS * 256 : 1];
-    v8bf16 qf[2][KM];
-    int token[2];  // of this lane's query rows; -1: none
-    __shared__ float slopes[PT_TILE];
-#pragma unroll
-    for (int rt = 0; rt < 2; ++rt) {
-        const int row = row0 + rt * 32 + l32, i = row / G, head = job.kvh * G + row % G;
-        const bool mine = row < R;
-        token[rt] = mine ? i : -1;
-        if (h == 0) slopes[wv * PT_ROWS + rt * 32 + l32] = mine && a.slopes ? a.slopes[head] * LOG2E : 0.0f;
-        const bf16_t* qp = a.q + ((size_t)(r.t0 + (mine ? i : 0)) * a.q_heads + (mine ? head : 0)) * HD + h * 8;
+    // The wave's query rows, a lane's (and lane ^ 32's) one, as B operands.
+    const int row0 = job.tile * PT_TILE + wv * 32, row = row0 + l32, token = row < R ? row / G : -1, head = job.kvh * G + row % G;
+    if (h == 0) slopes[wv * 32 + l32] = token >= 0 && a.slopes ? a.slopes[head] * LOG2E : 0.0f;
+    // For heads of 256 the first QS of them wait in LDS: with all in registers the loop would reload something from scratch memory,
+    // each time behind every load under way.
+    constexpr int QS = HD > 128 ? 4 : 0;
+    __shared__ __attribute__((aligned(16))) v8bf16 q_wait[QS ? QS * 512 : 1];
+    v8bf16 qf[KM];
+    {
+        const bf16_t* qp = a.q + ((size_t)(r.t0 + max(token, 0)) * a.q_heads + (token >= 0 ? head : 0)) * HD + h * 8;
 #pragma unroll
         for (int m = 0; m < KM; ++m) {
             v8bf16 x = *(const v8bf16*)(qp + m * 16);
-            if (!mine) x = (v8bf16)(__bf16)0.0f;
-            if (rt && m < QS)
-                q_wait[m * 256 + threadIdx.x] = x;
+            if (token < 0) x = (v8bf16)(__bf16)0.0f;
+            if (m < QS)
+                q_wait[m * 512 + threadIdx.x] = x;
             else
-                qf[rt][m] = x;
+                qf[m] = x;
         }
     }
-    const PagedSight early = paged_sight(a, r, prefix, min(row0, R - 1) / G), late = paged_sight(a, r, prefix, min(row0 + PT_ROWS - 1, R - 1) / G);
-    const int lo_whole = uniform(late.lo), hi_whole = uniform(early.hi);
+    const int lo_whole = uniform(paged_sight(a, r, prefix, min(row0 + 31, R - 1) / G).lo), hi_whole = uniform(paged_sight(a, r, prefix, min(row0, R - 1) / G).hi);
 
-    // This thread's pieces of a tile: piece i is position group gi's, 16 dims of one key and 16 positions of one value dim.
-    uint4 rk[NI], rv[NI];
-    int id[NI], found[NI], ks[NI], vs[NI];  // this tile's pages; the next one's as read; scale bytes
-    const int c0 = EITHER ? threadIdx.x & 127 : threadIdx.x, vg0 = uniform(c0 / HD);
-    // A tile's page numbers are read a tile before its keys and values, so that no load waits for another.
-    auto look = [&](int T) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            found[i] = table[min((T * TILE + (vg0 + i) * 16) >> shift, a.r.max_pages - 1)];
+    // This thread's pieces of a tile: 16 dims of one key and 16 positions of one value dim, in position group vg0 (of 16).
+    const bool keys = BOTH || wv * 64 < PIECES, vals = BOTH || (wv * 64 >= PIECES && wv * 64 < 2 * PIECES);
+    const int c0 = (int)threadIdx.x & (PIECES - 1), vg0 = uniform(c0 / HD);
+    uint4 rk, rv;
+    int id, found, ks, vs;  // this tile's page; the next one's as read; scale bytes
+    // A tile's page number is read a tile before its keys and values, so that no load waits for another.
+    auto look = [&](int T) __attribute__((always_inline)) { found = table[min((T * 32 + vg0 * 16) >> shift, a.r.max_pages - 1)]; };
+    auto load = [&](int T) __attribute__((always_inline)) {
+        const int p = T * 32 + vg0 * 16;
+        id = uniform(found);
+        id = ((id < a.c.pages) & (p >> shift < a.r.max_pages)) ? id : -1;
+        const size_t hd = (size_t)max(id, 0) * Hkv + job.kvh, at = (hd * ps + (p & (ps - 1))) * HD + c0 % HD * 16;
+        if constexpr (BOTH) {
+            ks = a.c.k_scale[hd];
+            vs = a.c.v_scale[hd];
+            rk = *(const uint4*)(a.c.k + at);
+            rv = *(const uint4*)(a.c.v + at);
+        } else {
+            ks = (keys ? a.c.k_scale : a.c.v_scale)[hd];
+            rk = *(const uint4*)((keys ? a.c.k : a.c.v) + at);
         }
     };
-    auto load = [&](int T, int i) __attribute__((always_inline)) {
-        {
-            id[i] = uniform(found[i]);
-            id[i] = ((id[i] < a.c.pages) & ((T * TILE + (vg0 + i) * 16) >> shift < a.r.max_pages)) ? id[i] : -1;
-            const size_t head = (size_t)max(id[i], 0) * Hkv + job.kvh, at = (head * ps + ((T * TILE + (vg0 + i) * 16) & (ps - 1))) * HD;
-            if constexpr (EITHER) {
-                ks[i] = (wv < 2 ? a.c.k_scale : a.c.v_scale)[head];
-                rk[i] = *(const uint4*)((wv < 2 ? a.c.k : a.c.v) + at + c0 % HD * 16);
-            } else {
-                ks[i] = a.c.k_scale[head];
-                vs[i] = a.c.v_scale[head];
-                rk[i] = *(const uint4*)(a.c.k + at + c0 % HD * 16);
-                rv[i] = *(const uint4*)(a.c.v + at + c0 % HD * 16);
-            }
-        }
-    };
-    // Step x of widening the loaded tile T into its buffer, or half of that: half of a piece. Keys: row (position), its 16-byte chunks spread
-    // over the banks; values: per dim 32 positions, likewise.
+    // Step x of widening the loaded tile T into its buffer. Keys: row (position), its 16-byte chunks spread over the banks;
+    // values: per dim 32 positions, likewise.
     const uint32_t lds0 = (uint32_t)(uintptr_t)LDS_PTR(&ring[0]);
     const int kp0 = c0 / (HD / 16), kc0 = c0 % (HD / 16) * 2, vd0 = c0 % HD;
     const uint32_t put_k = kp0 * HD * 2 + ((kc0 ^ (HD > 64 ? kp0 & 15 : (kp0 >> 1) & 7)) << 4);
     const uint32_t put_v = HALF + vd0 * 64 + ((vg0 * 2 ^ ((vd0 >> 1) & 3) ^ ((vd0 >> 3) & 1)) << 4);
-    auto put = [&](uint32_t at, v8bf16 x) __attribute__((always_inline)) { *(__attribute__((address_space(3))) v8bf16*)(uintptr_t)at = x; };
-    v8bf16 piece;
-    auto widen = [&](int T, int x, int half = -1) __attribute__((always_inline)) {
+    auto widen = [&](int T, int x) __attribute__((always_inline)) {
         const uint32_t buf = lds0 + T % 3 * BUF;
-        const int i = EITHER ? 0 : x >> 2, u = x & 1;
-        if (x == 0 && half < 1) {
+        const int u = x & 1;
+        const bool key = BOTH ? x < 2 : keys;
+        if (x == 0) {
             // Bytes that no token wrote may be anything, and so may those of a page that is not there.
-            bool tail = T * TILE + TILE > total;
+            if ((T * 32 + 32 > total) | (id < 0)) {
+                const int left = id < 0 ? 0 : total - (T * 32 + vg0 * 16);
+                uint32_t* w4 = (uint32_t*)(BOTH ? &rv : &rk);
+                if (vals)
 #pragma unroll
-            for (int k = 0; k < NI; ++k) tail |= id[k] < 0;
-            if (tail) {
-#pragma unroll
-                for (int k = 0; k < NI; ++k) {
-                    const int left = id[k] < 0 ? 0 : total - (T * TILE + (vg0 + k) * 16);
-                    uint32_t* w = (uint32_t*)(EITHER ? &rk[k] : &rv[k]);
-                    if (!EITHER || wv >= 2)
-#pragma unroll
-                        for (int y = 0; y < 4; ++y) w[y] &= left >= 4 * y + 4 ? 0xffffffffu : left <= 4 * y ? 0u : (1u << 8 * (left - 4 * y)) - 1;
-                }
+                    for (int y = 0; y < 4; ++y) w4[y] &= left >= 4 * y + 4 ? 0xffffffffu : left <= 4 * y ? 0u : (1u << 8 * (left - 4 * y)) - 1;
             }
-#pragma unroll
-            for (int k = 0; k < NI; ++k)
-                if (vd0 == 0) lost[T % 3][vg0 + k] = id[k] < 0;
+            if (vd0 == 0) lost[T % 3][vg0] = id < 0;
         }
-        const bool key = EITHER ? wv < 2 : !(x & 2);
-        const uint4 w = EITHER || key ? rk[i] : rv[i];
-        const float scale = paged_scale(EITHER || key ? ks[i] : vs[i]);
-        if (half < 1) piece = __builtin_shufflevector(paged_widen2(u ? w.z : w.x, scale), paged_widen2(u ? w.z : w.x, scale), 0, 1, 2, 3, -1, -1, -1, -1);
-        if (half != 0) {
-            const v4bf16 last = paged_widen2(u ? w.w : w.y, scale);
-            const uint32_t at = key ? i * (256 / (HD / 16) * HD * 2) + (put_k ^ (u << 4)) : put_v ^ (i << 5) ^ (u << 4);
-            put(buf + at, __builtin_shufflevector(__builtin_shufflevector(piece, piece, 0, 1, 2, 3), last, 0, 1, 2, 3, 4, 5, 6, 7));
-        }
+        const uint4 w4 = !BOTH || key ? rk : rv;
+        const uint32_t at = key ? put_k ^ (u << 4) : put_v ^ (u << 4);
+        if (keys | vals)
+            *(__attribute__((address_space(3))) v8bf16*)(uintptr_t)(buf + at) =
+                u ? paged_widen(w4.z, w4.w, paged_scale(!BOTH || key ? ks : vs)) : paged_widen(w4.x, w4.y, paged_scale(!BOTH || key ? ks : vs));
     };
 
     const int kp = (l32 & ~12) | (l32 & 4) << 1 | (l32 & 8) >> 1;  // the position of this lane's key row
     const uint32_t kl = kp * HD * 2 + ((h ^ (HD > 64 ? kp & 15 : (kp >> 1) & 7)) << 4);
     const uint32_t vl = HALF + l32 * 64 + ((h ^ ((l32 >> 1) & 3) ^ ((l32 >> 3) & 1)) << 4);
-    v16f o[2][VD], s[2];
+    v16f o[VD], s;
     typedef uint32_t u4_ __attribute__((ext_vector_type(4)));
-    u4_ pw[2][2];
+    u4_ pw[2];
     // Scores in powers of two: times scale log2 e beside the exponential, or capped and biased (`bent`) before the maxima.
     const bool bent = a.cap > 0.0f || a.slopes;
     const float mul = bent ? 1.0f : a.scale * LOG2E;
-    // What a query row's weights are relative to is the largest score of the first sub-block that it sees anything of, and
-    // stays: floats hold weights of up to 2^LEAP as exactly as others. Only if some score leaps further than that are the item's
-    // sums formed again, relative to the largest score, which is known by then. (Raising it on the way costs the loop
-    // copies of the sums even where it never happens: the compiler keeps them out of the MFMAs' registers for it.)
+    // What a query row's weights are relative to is the largest score of the first tile that it sees anything of, and stays:
+    // floats hold weights of up to 2^LEAP as exactly as others. Only if some score leaps further than that are the item's sums
+    // formed again, relative to the largest score, which is known by then. (Raising it on the way costs the loop copies of the
+    // sums even where it never happens: the compiler keeps them out of the MFMAs' registers for it.)
     constexpr float LEAP = 40.0f, UNSEEN = -3e38f;
-    float top[2] = {UNSEEN, UNSEEN}, most[2] = {-INFINITY, -INFINITY}, sum[2];
-
+    float top = UNSEEN, most = -INFINITY, sum;
     bool unseen = true;  // some row's reference is not known yet
     // The largest of three, NaN ones passed over.
     auto max3 = [](float x, float y, float z) __attribute__((always_inline)) {
@@ -697,200 +672,137 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PT_PER_CU(H
         asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(x), "v"(y), "v"(z));
         return m;
     };
-    // Scores of sub-block n, with the loaded tile (n + 1) widened beside their MFMAs; then what the weights are relative to.
-    auto scores = [&](int n) __attribute__((always_inline)) {
-        const uint32_t ka = lds0 + n % 3 * BUF + kl;
-        const int gone0 = lost[n % 3][0], gone1 = lost[n % 3][1];
-        v8bf16 kf[DEEP], qx[2];
+    // Scores of tile T, with the loaded tile T + 1 widened beside their MFMAs and the one after it asked for; then its weights.
+    auto scores = [&](int T) __attribute__((always_inline)) {
+        const uint32_t ka = lds0 + T % 3 * BUF + kl;
+        const int gone0 = lost[T % 3][0], gone1 = lost[T % 3][1];
+        v8bf16 kf[DEEP], qx[DEEP];
+        v16f c[CHAINS], zero;
 #pragma unroll
-        for (int m = 0; m < DEEP; ++m) kf[m] = paged_frag(ka ^ (m << 5));
+        for (int e = 0; e < 16; ++e) zero[e] = 0.0f;
 #pragma unroll
-        for (int m = 0; m < 2 && m < QS; ++m) qx[m] = q_wait[m * 256 + threadIdx.x];
+        for (int m = 0; m < DEEP; ++m) {
+            kf[m] = paged_frag(ka ^ (m << 5));
+            if (m < QS) qx[m] = q_wait[m * 512 + threadIdx.x];
+        }
 #pragma unroll
         for (int m = 0; m < KM; ++m) {
-            const v8bf16 q1 = m < QS ? qx[m & 1] : qf[1][m];
             __builtin_amdgcn_sched_barrier(0);
-            if (m)
-                asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(s[0]) : "v"(kf[m % DEEP]), "v"(qf[0][m]));
-            else
-                asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(s[0]) : "v"(kf[m % DEEP]), "v"(qf[0][m]));
-            const int x = m - (KM - STEPS);
-            if (x >= 0) widen(n + 1, x, 0);
-            __builtin_amdgcn_sched_barrier(0);
-            if (m)
-                asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(s[1]) : "v"(kf[m % DEEP]), "v"(q1));
-            else
-                asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(s[1]) : "v"(kf[m % DEEP]), "v"(q1));
-            if (m + 2 < QS) qx[m & 1] = q_wait[(m + 2) * 256 + threadIdx.x];
+            const v8bf16 q = m < QS ? qx[m % DEEP] : qf[m];
+            c[m % CHAINS] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[m % DEEP], q, m < CHAINS ? zero : c[m % CHAINS], 0, 0, 0);
+            if (m + DEEP < QS) qx[m % DEEP] = q_wait[(m + DEEP) * 512 + threadIdx.x];
             if (m + DEEP < KM) kf[m % DEEP] = paged_frag(ka ^ ((m + DEEP) << 5));
-            if (x >= 0) widen(n + 1, x, 1);
+            if (m >= KM - STEPS) widen(T + 1, m - (KM - STEPS));
         }
         __builtin_amdgcn_sched_barrier(0);
-        asm volatile("s_nop 15\n\ts_nop 15" : "+v"(s[0]), "+v"(s[1]));  // the last products' way into the registers
-        const int p0 = n * 32;
-        const int lost0 = uniform(gone0), lost1 = uniform(gone1);
-        if (bent) {
+        load(min(T + 2, T1 - 1));
+        look(min(T + 3, T1 - 1));
+        s = CHAINS > 1 ? c[0] + c[CHAINS - 1] : c[0];
+        const int p0 = T * 32, lost0 = uniform(gone0), lost1 = uniform(gone1);
+        if (bent)
 #pragma unroll
-            for (int rt = 0; rt < 2; ++rt)
+            for (int k = 0; k < 2; ++k) {  // the lane's positions: 8 from p0 + 16 k + 8 h on
+                float y[8];
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {  // the lane's positions: 8 from p0 + 16 k + 8 h on
-                    float y[8];
+                for (int e = 0; e < 8; ++e) y[e] = s[8 * k + e];
+                paged_scores<8>(a, y, slopes[wv * 32 + l32], p0 + 16 * k + 8 * h, r.p0 + token);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) y[e] = s[rt][8 * k + e];
-                    paged_scores<8>(a, y, slopes[wv * PT_ROWS + rt * 32 + l32], p0 + 16 * k + 8 * h, r.p0 + token[rt]);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) s[rt][8 * k + e] = y[e];
-                }
-        }
+                for (int e = 0; e < 8; ++e) s[8 * k + e] = y[e];
+            }
         if (!((p0 >= lo_whole) & (p0 + 32 <= hi_whole) & !(lost0 | lost1))) {
+            const PagedSight see = paged_sight(a, r, prefix, max(token, 0));
+            const int lo = see.lo - p0 - 8 * h, hi = token < 0 ? -64 : see.hi - p0 - 8 * h;
 #pragma unroll
-            for (int rt = 0; rt < 2; ++rt) {
-                const PagedSight see = paged_sight(a, r, prefix, max(token[rt], 0));
-                const int lo = see.lo - p0 - 8 * h, hi = token[rt] < 0 ? -64 : see.hi - p0 - 8 * h;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int p = 16 * (e >> 3) + (e & 7);
-                    const float x = (e >> 3 ? lost1 : lost0) ? QNAN : s[rt][e];
-                    s[rt][e] = ((p < lo) | (p >= hi)) ? -INFINITY : x;
-                }
+            for (int e = 0; e < 16; ++e) {
+                const int p = 16 * (e >> 3) + (e & 7);
+                const float x = (e >> 3 ? lost1 : lost0) ? QNAN : s[e];
+                s[e] = ((p < lo) | (p >= hi)) ? -INFINITY : x;
             }
         }
+        float m = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) m = max3(s[e], s[e + 1], m);
+        most = fmaxf(most, m);
         if (unseen) {
+            m = fmaxf(m, __shfl_xor(m, 32)) * mul;
+            top = ((top == UNSEEN) & (m > -INFINITY)) ? m : top;
+            unseen = __any(top == UNSEEN);
+        }
 #pragma unroll
-            for (int rt = 0; rt < 2; ++rt) {
-                float m = -INFINITY;
-#pragma unroll
-                for (int e = 0; e < 16; e += 2) m = max3(s[rt][e], s[rt][e + 1], m);
-                m = fmaxf(m, __shfl_xor(m, 32)) * mul;
-                top[rt] = ((top[rt] == UNSEEN) & (m > -INFINITY)) ? m : top[rt];
-            }
-            unseen = __any((top[0] == UNSEEN) | (top[1] == UNSEEN));
+        for (int e = 0; e < 16; e += 2) {
+            const float p = exp2_(__builtin_fmaf(s[e], mul, -top)), q = exp2_(__builtin_fmaf(s[e + 1], mul, -top));
+            sum += p;
+            sum += q;
+            pw[e >> 3][(e >> 1) & 3] = pk_bf16(p, q);
         }
     };
-    // Weight x of the lane's 32.
-    float even;
-    auto weight = [&](int x, u4_ (&w)[2][2]) __attribute__((always_inline)) {
-        const int rt = x >> 4, e = x & 15;
-        const float p = exp2_(__builtin_fmaf(s[rt][e], mul, -top[rt]));
-        sum[rt] += p;
-        if (e & 1) {
-            most[rt] = max3(s[rt][e - 1], s[rt][e], most[rt]);
-            uint32_t both = pk_bf16(even, p);
-            asm volatile("" : "+v"(both));  // here, beside the MFMAs, not where it is first used
-            w[rt][e >> 3][(e >> 1) & 3] = both;
-        }
-        even = p;
-    };
-    // Weights x V of sub-block n, beside them the next one's weights.
-    auto values = [&](int n, auto next) __attribute__((always_inline)) {
-        __builtin_amdgcn_sched_barrier(0);
-        const uint32_t va = lds0 + n % 3 * BUF + vl;
-        auto frag = [&](int x) __attribute__((always_inline)) { return paged_frag((va ^ ((x & 1) << 5)) + (x >> 1) * 2048); };
+    // Weights x V of tile T.
+    auto values = [&](int T) __attribute__((always_inline)) {
+        const uint32_t va = lds0 + T % 3 * BUF + vl;
+        auto frag = [&](int x) __attribute__((always_inline)) { return paged_frag((va ^ (x / VD << 5)) + x % VD * 2048); };
         v8bf16 vf[DEEP];
 #pragma unroll
         for (int x = 0; x < DEEP; ++x) vf[x] = frag(x);
-        u4_ nw[2][2];
 #pragma unroll
         for (int x = 0; x < 2 * VD; ++x) {
-            // A wave's own instructions run beside an MFMA only until the next one: they go between the two of a step as well.
-#pragma unroll
-            for (int rt = 0; rt < 2; ++rt) {
-                __builtin_amdgcn_sched_barrier(0);
-                o[rt][x >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[x % DEEP], __builtin_bit_cast(v8bf16, pw[rt][x & 1]), o[rt][x >> 1], 0, 0, 0);
-                __builtin_amdgcn_sched_barrier(0);
-                if (rt && x + DEEP < 2 * VD) vf[x % DEEP] = frag(x + DEEP);
-                if constexpr (decltype(next)::value) {
-                    if (rt && x < NI) load(min(n + 3, T1 - 1), x);
-                    if (rt && x == NI) look(min(n + 4, T1 - 1));
-#pragma unroll
-                    for (int y = 0; y < 8 / VD; ++y) weight((2 * x + rt) * (8 / VD) + y, nw);
-                }
-            }
+            __builtin_amdgcn_sched_barrier(0);
+            o[x % VD] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[x % DEEP], __builtin_bit_cast(v8bf16, pw[x / VD]), o[x % VD], 0, 0, 0);
+            if (x + DEEP < 2 * VD) vf[x % DEEP] = frag(x + DEEP);
         }
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (decltype(next)::value) {
-#pragma unroll
-            for (int rt = 0; rt < 2; ++rt)
-#pragma unroll
-                for (int ks2 = 0; ks2 < 2; ++ks2) pw[rt][ks2] = nw[rt][ks2];
-        }
     };
+    // A tile's beginning: what the waves have widened is in LDS.
+    auto meet = [&]() __attribute__((always_inline)) { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
 
     for (int pass = 0;; ++pass) {
+        sum = 0.0f;
 #pragma unroll
-        for (int rt = 0; rt < 2; ++rt) {
-            sum[rt] = 0.0f;
+        for (int d = 0; d < VD; ++d)
 #pragma unroll
-            for (int d = 0; d < VD; ++d)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) o[rt][d][e] = 0.0f;
-        }
+            for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
         if (T0 >= T1) break;
-        auto load_all = [&](int T) __attribute__((always_inline)) {
-#pragma unroll
-            for (int i = 0; i < NI; ++i) load(T, i);
-        };
         look(T0);
-        load_all(T0);
+        load(T0);
         look(min(T0 + 1, T1 - 1));
 #pragma unroll
         for (int x = 0; x < STEPS; ++x) widen(T0, x);
-        load_all(min(T0 + 1, T1 - 1));
+        load(min(T0 + 1, T1 - 1));
         look(min(T0 + 2, T1 - 1));
-        // Tile T is in buffer T % 3. A tile is widened into the buffer of the one three before, whose last weights x V every
-        // wave has behind it when it comes to the barrier that a tile begins with. The tile after it is loaded as soon as its
-        // registers are free: most of a tile's time before it is widened.
+        // Tile T is in buffer T % 3, widened there before its beginning, which the first four waves meet before their scores of it, the
+        // other four, which share the SIMDs with them, before their weights x V of the tile before: so one of a SIMD's two waves
+        // forms weights while the other feeds the matrix cores. A tile goes into the buffer of the one three before, whose
+        // last weights x V lie before the meeting before.
         for (int T = T0; T < T1; ++T) {
-            __syncthreads();
+            if (wv < 4 || T == T0) meet();
             scores(T);
-            if (T > T0) {
-                values(T - 1, std::true_type{});
-            } else {
-#pragma unroll
-                for (int x = 0; x < 32; ++x) weight(x, pw);
-                load_all(min(T0 + 2, T1 - 1));
-                look(min(T0 + 3, T1 - 1));
-            }
+            if (wv >= 4 && T + 1 < T1) meet();
+            values(T);
         }
-        values(T1 - 1, std::false_type{});
-        bool leapt = false;
-#pragma unroll
-        for (int rt = 0; rt < 2; ++rt) {
-            most[rt] = fmaxf(most[rt], __shfl_xor(most[rt], 32)) * mul;
-            leapt |= most[rt] > top[rt] + LEAP;
-        }
-        if (pass || !__syncthreads_or(leapt)) break;
-#pragma unroll
-        for (int rt = 0; rt < 2; ++rt) top[rt] = fmaxf(top[rt], most[rt]);
+        most = fmaxf(most, __shfl_xor(most, 32)) * mul;
+        if (pass || !__syncthreads_or(most > top + LEAP)) break;
+        top = fmaxf(top, most);
     }
 
+    const float l = sum + __shfl_xor(sum, 32);
     if (alone) {
-#pragma unroll
-        for (int rt = 0; rt < 2; ++rt) {
-            const float l = sum[rt] + __shfl_xor(sum[rt], 32), inv = r.skip ? 0.0f : 1.0f / l;
-            const int row = row0 + rt * 32 + l32;
-            if (row >= R) continue;
-            bf16_t* out = a.out + ((size_t)(r.t0 + row / G) * a.q_heads + job.kvh * G + row % G) * HD + h * 4;
+        const float inv = r.skip ? 0.0f : 1.0f / l;
+        if (token >= 0) {
+            bf16_t* out = a.out + ((size_t)(r.t0 + token) * a.q_heads + head) * HD + h * 4;
 #pragma unroll
             for (int d = 0; d < VD; ++d)
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
-                    *(uint2*)(out + d * 32 + q * 8) = make_uint2(pk_bf16(o[rt][d][4 * q] * inv, o[rt][d][4 * q + 1] * inv),
-                                                                 pk_bf16(o[rt][d][4 * q + 2] * inv, o[rt][d][4 * q + 3] * inv));
+                    *(uint2*)(out + d * 32 + q * 8) = make_uint2(pk_bf16(o[d][4 * q] * inv, o[d][4 * q + 1] * inv), pk_bf16(o[d][4 * q + 2] * inv, o[d][4 * q + 3] * inv));
         }
     } else {
-    // [slot][wave][rt][d][q][lane] of four dims, then per query row its maximum and sum.
-    float* part = (float*)(a.scratch + a.plan.cut_part) + (size_t)slot * (PT_TILE * (HD + 2));
-#pragma unroll
-    for (int rt = 0; rt < 2; ++rt) {
-        const float l = sum[rt] + __shfl_xor(sum[rt], 32);
-        if (h == 0) *(float2*)(part + PT_TILE * HD + (wv * PT_ROWS + rt * 32 + l32) * 2) = make_float2(top[rt], l);
+        // [slot][wave][d][q][lane] of four dims, then per query row what its weights are relative to and their sum.
+        float* part = (float*)(a.scratch + a.plan.cut_part) + (size_t)slot * (PT_TILE * (HD + 2));
+        if (h == 0) *(float2*)(part + PT_TILE * HD + (wv * 32 + l32) * 2) = make_float2(top, l);
 #pragma unroll
         for (int d = 0; d < VD; ++d)
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-                *(v4f*)(part + ((((wv * 2 + rt) * VD + d) * 4 + q) * 64 + lane) * 4) = (v4f){o[rt][d][4 * q], o[rt][d][4 * q + 1], o[rt][d][4 * q + 2], o[rt][d][4 * q + 3]};
-    }
+                *(v4f*)(part + (((wv * VD + d) * 4 + q) * 64 + lane) * 4) = (v4f){o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]};
     }
     __syncthreads();  // the ring and the slopes are the next tile's
     }
@@ -989,7 +901,7 @@ hipError_t q38_paged_attention(const PagedAttnArgs& a, hipStream_t stream) {
     }
 #define TILES(HD)                                                                                                             \
     do {                                                                                                                     \
-        hipLaunchKernelGGL((paged_tiles_kernel<HD>), dim3(a.plan.tiles), dim3(256), 0, stream, a);                           \
+        hipLaunchKernelGGL((paged_tiles_kernel<HD>), dim3(a.plan.tiles), dim3(512), 0, stream, a);                           \
         if (a.plan.parts) hipLaunchKernelGGL((paged_join_tiles_kernel<HD>), dim3(a.plan.cut_jobs * 8 * (HD / 32)), dim3(256), 0, stream, a); \
     } while (0)
     switch (a.c.head_dim) {
