@@ -458,7 +458,7 @@ struct PagedWork {
 
 // The tile that unit u of the call's work is in, and its first unit.
 struct PagedJob {
-    int row, tile, kvh, index;
+    int row, tile, kvh;
     long long start;
     int units;
 };
@@ -468,12 +468,12 @@ __device__ __forceinline__ long long uniform(long long x) {
 }
 
 // Goes over the tiles, a lane for each: 64 rows' numbers of tiles at a time, then 64 of their tiles, whose rows the lanes look up among
-// them. Without `find` it returns the work's total of sub-blocks per KV head, number of tiles and longest tile in job.start, index and units; with it
+// them. Without `find` it returns the work's total of sub-blocks per KV head, number of tiles and longest tile in job.start, tile and units; with it
 // the job of unit u.
 __device__ __forceinline__ PagedJob paged_tiles_list(const PagedAttnArgs& a, int G, bool find, long long u, bool whole) {
     const int lane = threadIdx.x & 63, Hkv = a.c.kv_heads;
     long long before = 0;
-    int index = 0, longest = 1;
+    int tiles = 0, longest = 1;
     for (int base = 0; base < a.r.rows; base += 64) {
         const int at = min(base + lane, a.r.rows - 1);
         PagedRow r = paged_row(a.r, at, a.c.page_size);
@@ -517,27 +517,26 @@ __device__ __forceinline__ PagedJob paged_tiles_list(const PagedAttnArgs& a, int
                 const long long first = before + uniform(__shfl(sum - units, f)) * Hkv;
                 job.kvh = (int)((u - first) / job.units);
                 job.start = first + (long long)job.kvh * job.units;
-                job.index = (index + k0 + f) * Hkv + job.kvh;
                 return job;
             }
             before += uniform(__shfl(sum, 63)) * (find ? Hkv : 1);
         }
-        index += count;
+        tiles += count;
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) longest = max(longest, __shfl_xor(longest, o));
-    return {-1, 0, 0, index, before, uniform(longest)};
+    return {-1, tiles, 0, before, uniform(longest)};
 }
 
 __device__ __forceinline__ PagedWork paged_work(const PagedAttnArgs& a, int G) {
     const PagedJob all = paged_tiles_list(a, G, false, 0, false);
-    const int jobs = all.index * a.c.kv_heads;
+    const int jobs = all.tile * a.c.kv_heads;
     const long long total = all.start * a.c.kv_heads;
     if (!a.plan.parts || jobs >= PT_FEW * a.plan.cus || all.units <= 2 * PT_LEAST) return {jobs, jobs, jobs, true};
     return {total, jobs, (int)max(1LL, min((long long)a.plan.parts, total / PT_LEAST)), false};
 }
 
-// A cut tile in the scratch's table: which workgroups' sums make it.
+// A cut tile in the scratch's table, at the workgroup that begins it: which workgroups' sums make it.
 struct PagedCut {
     int row, tile, kvh, slot, first, last;  // slot: where the first one's are; a later workgroup w's are in slot 2 w
 };
@@ -545,7 +544,7 @@ struct PagedCut {
 }  // namespace
 
 template <int HD>
-__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_tiles_kernel(const PagedAttnArgs a) {
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2 * PT_PER_CU(HD), 2 * PT_PER_CU(HD)))) void paged_tiles_kernel(const PagedAttnArgs a) {
     constexpr int KM = HD / 16, VD = HD / 32, HALF = 32 * HD * 2, BUF = 2 * HALF;  // MFMA steps; bytes of a buffer's keys, of a buffer
     constexpr int PIECES = 2 * HD;       // 16-byte pieces of a tile's keys, and of its values: one of each per thread, or of either
     constexpr bool BOTH = HD == 256;
@@ -558,8 +557,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int lane = threadIdx.x & 63, wv = uniform((int)threadIdx.x >> 6), l32 = lane & 31, h = lane >> 5;
     const int Hkv = a.c.kv_heads, G = a.q_heads / Hkv, ps = a.c.page_size, shift = __builtin_ctz(ps);
     const PagedWork work = paged_work(a, G);
-    if (blockIdx.x == 0 && threadIdx.x == 0 && a.plan.parts) *(int*)(a.scratch + a.plan.cuts) = work.whole ? 0 : work.jobs;
     const int w = blockIdx.x;
+    if (w == 0 && threadIdx.x == 0 && a.plan.parts) *(int*)(a.scratch + a.plan.cuts) = work.whole || !work.jobs ? 0 : work.parts;
     if (!work.jobs || w >= work.parts) return;
     const long long begin = work.start(w), end = work.start(w + 1);
     for (long long unit = begin; unit < end;) {
@@ -574,8 +573,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int T0 = span.lo + (work.whole ? 0 : (int)(unit - job.start)), T1 = work.whole ? span.hi : min(span.hi, span.lo + (int)(stop - job.start));
     const bool alone = unit == job.start && stop == job.start + job.units;
     const int slot = 2 * w + (unit > begin);
-    if (unit == job.start && !work.whole && threadIdx.x == 0)
-        ((PagedCut*)(a.scratch + a.plan.cuts + 256))[job.index] = {job.row, job.tile, job.kvh, slot, w, alone ? w : work.part(job.start + job.units - 1)};
+    // The tile that this part begins and others end: this part's last, at most one.
+    if (stop == end && !work.whole && threadIdx.x == 0)
+        ((PagedCut*)(a.scratch + a.plan.cuts + 256))[w] = {job.row, job.tile, job.kvh, slot, w, unit == job.start && !alone ? work.part(job.start + job.units - 1) : w};
     unit = stop;
 
     // The wave's query rows, a lane's (and lane ^ 32's) one, as B operands.
@@ -808,7 +808,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
 }
 
-// The parts of cut tiles put together. Grid: tiles x the tile's eight groups of 32 query rows x dims in blocks of 32.
+// The parts of cut tiles put together. Grid: parts (the tile that each begins, if it is cut) x the tile's eight groups of 32 query rows x dims in blocks of 32.
 template <int HD>
 __global__ __launch_bounds__(256) void paged_join_tiles_kernel(const PagedAttnArgs a) {
     constexpr int VD = HD / 32;
@@ -864,9 +864,8 @@ PagedPlan paged_attention_plan(const PagedCache& c, const PagedRows& r, int q_he
         p.parts = many && !r.q_start ? 0 : (int)std::min<long long>(p.cus * PT_PER_CU(c.head_dim), std::max<long long>(1, jobs * blocks / PT_LEAST));
         p.tiles = (int)std::max<long long>(p.parts, jobs);
         if (p.parts) {
-            p.cut_jobs = (int)std::min<long long>(jobs, (long long)PT_FEW * p.cus);
             p.cuts = p.bytes + 255 & ~(size_t)255;
-            p.cut_part = p.cuts + 256 + (size_t)p.cut_jobs * sizeof(PagedCut) + 255 & ~(size_t)255;
+            p.cut_part = p.cuts + 256 + (size_t)p.parts * sizeof(PagedCut) + 255 & ~(size_t)255;
             p.bytes = p.cut_part + (size_t)2 * p.parts * PT_TILE * (c.head_dim + 2) * 4;
         }
     }
@@ -902,7 +901,7 @@ hipError_t q38_paged_attention(const PagedAttnArgs& a, hipStream_t stream) {
 #define TILES(HD)                                                                                                             \
     do {                                                                                                                     \
         hipLaunchKernelGGL((paged_tiles_kernel<HD>), dim3(a.plan.tiles), dim3(512), 0, stream, a);                           \
-        if (a.plan.parts) hipLaunchKernelGGL((paged_join_tiles_kernel<HD>), dim3(a.plan.cut_jobs * 8 * (HD / 32)), dim3(256), 0, stream, a); \
+        if (a.plan.parts) hipLaunchKernelGGL((paged_join_tiles_kernel<HD>), dim3(a.plan.parts * 8 * (HD / 32)), dim3(256), 0, stream, a); \
     } while (0)
     switch (a.c.head_dim) {
         case 64: TILES(64); break;
