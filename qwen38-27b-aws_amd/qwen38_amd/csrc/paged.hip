@@ -19,7 +19,9 @@ __device__ __forceinline__ int paged_need(float amax) {
     return min(max(b, 1), 254);
 }
 
-__device__ __forceinline__ uint32_t e4m3_byte(float x) { return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false) & 0xffu; }
+__device__ __forceinline__ uint32_t e4m3_four(float a, float b, float c, float d) {
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false), true);
+}
 
 // Four e4m3 codes times 2^-shift, coded again.
 __device__ __forceinline__ uint32_t e4m3_shift(uint32_t w, int shift) {
@@ -29,87 +31,120 @@ __device__ __forceinline__ uint32_t e4m3_shift(uint32_t w, int shift) {
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(ldexpf(b[0], -shift), ldexpf(b[1], -shift), lo, true);
 }
 
-// One head's vector in a wave, E = hd / 64 dims per lane: RMS norm with weight 1 + w (w null: none), then the rotation of its
-// first `rot` dims (dim d with d +- rot / 2, rot / 2 a multiple of E).
-template <int E>
-__device__ __forceinline__ void norm_rotate(float (&x)[E], const bf16_t* w, float eps, const bf16_t* cos, const bf16_t* sin, int rot, int lane,
-                                            bool& fine) {
-    constexpr int HD = E * 64;
-    if (w) {
+// How a wave holds head vectors: HD / 8 lanes each, eight dims per lane in two runs of four, from `lo` and from `hi`. The lanes of
+// the rotated dims hold both halves of their pairs, so that nothing moves between lanes.
+struct HeadLane {
+    int vec, lo, hi;  // the lane's vector of the wave's 64 / (HD / 8)
+    bool turns;
+};
+
+template <int HD>
+__device__ __forceinline__ HeadLane head_lane(int lane, int rot) {
+    const int i = lane % (HD / 8), n = rot / 8;  // the first n lanes: pairs
+    return i < n ? HeadLane{lane / (HD / 8), 4 * i, rot / 2 + 4 * i, true} : HeadLane{lane / (HD / 8), 8 * i, 8 * i + 4, false};
+}
+
+typedef uint32_t words2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ void load_dims(const bf16_t* p, const HeadLane& l, words2& lo, words2& hi) {
+    lo = *(const words2*)(p + l.lo);
+    hi = *(const words2*)(p + l.hi);
+}
+
+__device__ __forceinline__ void widen_dims(words2 lo, words2 hi, float (&x)[8]) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        x[2 * e] = lo_bf(lo[e]), x[2 * e + 1] = hi_bf(lo[e]);
+        x[4 + 2 * e] = lo_bf(hi[e]), x[5 + 2 * e] = hi_bf(hi[e]);
+    }
+}
+
+// RMS norm with weights 1 + w (gain: those; normed false: none), then the rotation. False if the norm is of something not
+// finite, the sum of the squares included: else large finite values would come out as zeros.
+template <int HD>
+__device__ __forceinline__ bool norm_rotate(float (&x)[8], bool normed, const float (&gain)[8], float eps, const HeadLane& l, const bf16_t* cos,
+                                            const bf16_t* sin) {
+    bool fine = true;
+    if (normed) {
         float ss = 0.0f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) ss += x[e] * x[e];
-        ss = warp_sum(ss);
-        fine = fine && ss < INFINITY;  // else the norm of large finite values would be zero
+        for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
+#pragma unroll
+        for (int o = 1; o < HD / 8; o <<= 1) ss += __shfl_xor(ss, o);
+        fine = ss < INFINITY;
         const float f = 1.0f / sqrtf(ss * (1.0f / HD) + eps);
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = x[e] * f * (1.0f + bf2f(w[lane * E + e]));
+        for (int e = 0; e < 8; ++e) x[e] = x[e] * f * gain[e];
     }
-    if (rot) {
-        const int half = rot / 2;
-        const bool low = lane * E < half;
-        const int other = low ? lane + half / E : lane - half / E;
+    if (l.turns) {
+        words2 a, b;
+        float c[8], s[8];
+        load_dims(cos, l, a, b);
+        widen_dims(a, b, c);
+        load_dims(sin, l, a, b);
+        widen_dims(a, b, s);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const float p = __shfl(x[e], other & 63);
-            const int d = lane * E + e;
-            if (d < rot) x[e] = x[e] * bf2f(cos[d]) + (low ? -p : p) * bf2f(sin[d]);
+        for (int e = 0; e < 4; ++e) {
+            const float lo = x[e], hi = x[4 + e];
+            x[e] = lo * c[e] - hi * s[e];
+            x[4 + e] = hi * c[4 + e] + lo * s[4 + e];
         }
     }
+    return fine;
 }
 
-template <int E>
-__device__ __forceinline__ void load_dims(const bf16_t* p, float (&x)[E]) {
-    if constexpr (E == 4) {
-        const uint2 w = *(const uint2*)p;
-        x[0] = lo_bf(w.x), x[1] = hi_bf(w.x), x[2] = lo_bf(w.y), x[3] = hi_bf(w.y);
-    } else if constexpr (E == 2) {
-        const uint32_t w = *(const uint32_t*)p;
-        x[0] = lo_bf(w), x[1] = hi_bf(w);
-    } else {
-        x[0] = bf2f(*p);
-    }
+__device__ __forceinline__ void load_gain(const bf16_t* w, const HeadLane& l, float (&gain)[8]) {
+    words2 lo = {}, hi = {};
+    if (w) load_dims(w, l, lo, hi);
+    widen_dims(lo, hi, gain);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) gain[e] += 1.0f;
 }
 
-constexpr int APPEND_TOKENS = 8;  // a wave's tokens of one page at most: their keys and values stay in its registers
-constexpr int APPEND_HEADS = 8;   // a wave's query heads of one token
+constexpr int APPEND_STEPS = 4;  // a lane's vectors of one page, or of the queries: all of them stay in its registers
+
+// Tokens of one page that a workgroup of nw waves has room for.
+constexpr int append_room(int head_dim, int nw) { return nw * (64 / (head_dim / 8)) * APPEND_STEPS; }
 
 }  // namespace
 
-// Grid: per row, page it may touch and KV head one workgroup; then the queries, a wave per token and APPEND_HEADS heads.
-// A workgroup has all of its page's new tokens, so the page's largest value is known before any of them is coded, and every
-// input is read once.
-template <int E, int NW>
+// Grid: per row, page it may touch and KV head one workgroup; then the queries, APPEND_STEPS vectors per lane. A workgroup has all
+// of its page's new tokens, so the page's largest value is known before any of them is coded, and every input is read once.
+// Bound: memory; for a few tokens a launch's and two loads' time.
+template <int HD, int NW>
 __global__ __launch_bounds__(NW * 64) void paged_append_kernel(const PagedAppendArgs a) {
-    constexpr int HD = E * 64;
+    constexpr int VECS = 64 / (HD / 8);  // vectors of a wave at a time
     __shared__ float amax[2][NW];
-    __shared__ __attribute__((aligned(16))) uint8_t codes[NW * APPEND_TOKENS * HD];  // the new values, [token][dim]
+    __shared__ __attribute__((aligned(16))) uint8_t codes[128 * HD];  // the new values, [token][dim]
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int Hkv = a.c.kv_heads, ps = a.c.page_size;
+    const HeadLane l = head_lane<HD>(lane, a.rot);
+    float gain[8];
     if ((int)blockIdx.x >= a.kv_blocks) {
-        const int groups = (a.q_heads + APPEND_HEADS - 1) / APPEND_HEADS, id = (blockIdx.x - a.kv_blocks) * NW + wv;
-        const int t = id / groups, h0 = id % groups * APPEND_HEADS;
-        const int tokens = a.r.q_start ? min(a.r.q_start[a.r.rows], a.r.tokens) : a.r.tokens;
-        if (t >= tokens) return;
-        float x[APPEND_HEADS][E];
+        const long long tokens = a.r.q_start ? min(a.r.q_start[a.r.rows], a.r.tokens) : a.r.tokens;
+        const long long first = ((long long)(blockIdx.x - a.kv_blocks) * NW + wv) * (VECS * APPEND_STEPS) + l.vec;
+        words2 lo[APPEND_STEPS], hi[APPEND_STEPS];
 #pragma unroll
-        for (int h = 0; h < APPEND_HEADS; ++h)
-            if (h0 + h < a.q_heads) load_dims<E>(a.q + t * a.q_token + (h0 + h) * a.q_head + lane * E, x[h]);
+        for (int i = 0; i < APPEND_STEPS; ++i) {
+            const long long u = first + i * VECS;
+            const int t = (int)(u / a.q_heads), h = (int)(u % a.q_heads);
+            lo[i] = hi[i] = (words2){0, 0};
+            if (t < tokens) load_dims(a.q + t * a.q_token + h * a.q_head, l, lo[i], hi[i]);
+        }
+        load_gain(a.q_norm, l, gain);
 #pragma unroll
-        for (int h = 0; h < APPEND_HEADS; ++h) {
-            if (h0 + h >= a.q_heads) break;
-            bool fine = true;
-            norm_rotate<E>(x[h], a.q_norm, a.eps, a.cos + (size_t)t * a.rot, a.sin + (size_t)t * a.rot, a.rot, lane, fine);
-            if (!fine)
+        for (int i = 0; i < APPEND_STEPS; ++i) {
+            const long long u = first + i * VECS;
+            const int t = (int)(u / a.q_heads), at = min(t, a.r.tokens - 1);
+            float x[8];
+            widen_dims(lo[i], hi[i], x);
+            if (!norm_rotate<HD>(x, a.q_norm != nullptr, gain, a.eps, l, a.cos + (size_t)at * a.rot, a.sin + (size_t)at * a.rot))
 #pragma unroll
-                for (int e = 0; e < E; ++e) x[h][e] = QNAN;
-            bf16_t* o = a.q_out + ((size_t)t * a.q_heads + h0 + h) * HD + lane * E;
-            if constexpr (E == 4)
-                *(uint2*)o = make_uint2(pk_bf16(x[h][0], x[h][1]), pk_bf16(x[h][2], x[h][3]));
-            else if constexpr (E == 2)
-                *(uint32_t*)o = pk_bf16(x[h][0], x[h][1]);
-            else
-                *o = f2bf(x[h][0]);
+                for (int e = 0; e < 8; ++e) x[e] = QNAN;
+            if (t < tokens) {
+                *(words2*)(a.q_out + u * HD + l.lo) = (words2){pk_bf16(x[0], x[1]), pk_bf16(x[2], x[3])};
+                *(words2*)(a.q_out + u * HD + l.hi) = (words2){pk_bf16(x[4], x[5]), pk_bf16(x[6], x[7])};
+            }
         }
         return;
     }
@@ -121,83 +156,83 @@ __global__ __launch_bounds__(NW * 64) void paged_append_kernel(const PagedAppend
     if (lo >= hi) return;
     const int id = paged_find(a.r, a.r.pages + (size_t)row * a.r.max_pages, page, a.c.pages);
     if (id < 0) return;
+    const size_t head = (size_t)id * Hkv + kvh, at = head * ps * HD;
+    const int k_old = a.c.k_scale[head], v_old = a.c.v_scale[head];
 
-    float k[APPEND_TOKENS][E], v[APPEND_TOKENS][E];
-    float km = 0.0f, vm = 0.0f;
+    float k[APPEND_STEPS][8], km = 0.0f, vm = 0.0f;
+    words2 w[APPEND_STEPS][4];  // the new keys and values
     const int t0 = r.t0 + base - r.p0;  // the token of slot 0
+    auto slot_of = [&](int i) { return lo + (i * NW + wv) * VECS + l.vec; };
 #pragma unroll
-    for (int i = 0; i < APPEND_TOKENS; ++i) {
-        const int slot = lo + i * NW + wv;
-        if (slot >= hi) continue;
-        const size_t t = t0 + slot;
-        load_dims<E>(a.k + t * a.k_token + kvh * a.k_head + lane * E, k[i]);
-        load_dims<E>(a.v + t * a.v_token + kvh * a.v_head + lane * E, v[i]);
+    for (int i = 0; i < APPEND_STEPS; ++i) {
+        if (lo + (i * NW + wv) * VECS >= hi) continue;
+        const size_t t = t0 + min(slot_of(i), hi - 1);
+        load_dims(a.k + t * a.k_token + kvh * a.k_head, l, w[i][0], w[i][1]);
+        load_dims(a.v + t * a.v_token + kvh * a.v_head, l, w[i][2], w[i][3]);
     }
+    load_gain(a.k_norm, l, gain);
 #pragma unroll
-    for (int i = 0; i < APPEND_TOKENS; ++i) {
-        const int slot = lo + i * NW + wv;
-        if (slot >= hi) continue;
-        const size_t t = t0 + slot;
-        bool fine = true;
-        norm_rotate<E>(k[i], a.k_norm, a.eps, a.cos + t * a.rot, a.sin + t * a.rot, a.rot, lane, fine);
+    for (int i = 0; i < APPEND_STEPS; ++i) {
+        if (lo + (i * NW + wv) * VECS >= hi) continue;
+        const size_t t = t0 + min(slot_of(i), hi - 1);  // past the last token: that one again
+        widen_dims(w[i][0], w[i][1], k[i]);
+        float v[8];
+        widen_dims(w[i][2], w[i][3], v);
+        int fine = norm_rotate<HD>(k[i], a.k_norm != nullptr, gain, a.eps, l, a.cos + t * a.rot, a.sin + t * a.rot);
         float ka = 0.0f, va = 0.0f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            fine = fine && fabsf(k[i][e]) < INFINITY && fabsf(v[i][e]) < INFINITY;
+        for (int e = 0; e < 8; ++e) {
+            fine &= (int)(fabsf(k[i][e]) < INFINITY) & (int)(fabsf(v[e]) < INFINITY);
             ka = fmaxf(ka, fabsf(k[i][e]));
-            va = fmaxf(va, fabsf(v[i][e]));
+            va = fmaxf(va, fabsf(v[e]));
         }
-        if (__all(fine)) {
+#pragma unroll
+        for (int o = 1; o < HD / 8; o <<= 1) fine &= __shfl_xor(fine, o);
+        if (fine) {
             km = fmaxf(km, ka);
             vm = fmaxf(vm, va);
         } else {
+            w[i][2] = w[i][3] = (words2){0, 0};
 #pragma unroll
-            for (int e = 0; e < E; ++e) k[i][e] = QNAN, v[i][e] = 0.0f;
+            for (int e = 0; e < 8; ++e) k[i][e] = QNAN;
         }
     }
     km = warp_max(km);
     vm = warp_max(vm);
     if (lane == 0) amax[0][wv] = km, amax[1][wv] = vm;
-    const size_t head = (size_t)id * Hkv + kvh, at = head * ps * HD;
-    const int k_old = a.c.k_scale[head], v_old = a.c.v_scale[head];
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < NW; ++w) km = fmaxf(km, amax[0][w]), vm = fmaxf(vm, amax[1][w]);
+    for (int j = 0; j < NW; ++j) km = fmaxf(km, amax[0][j]), vm = fmaxf(vm, amax[1][j]);
     int kb = paged_need(km), vb = paged_need(vm);
     if (lo > 0) {  // the page goes on: what it holds stays, coded again if the scale grows
         kb = max(kb, k_old);
         vb = max(vb, v_old);
         if (kb > k_old)
             for (int i = threadIdx.x; i < lo * HD / 4; i += NW * 64) {
-                uint32_t* w = (uint32_t*)(a.c.k + at) + i;
-                *w = e4m3_shift(*w, kb - k_old);
+                uint32_t* w4 = (uint32_t*)(a.c.k + at) + i;
+                *w4 = e4m3_shift(*w4, kb - k_old);
             }
         if (vb > v_old)
             for (int i = threadIdx.x; i < (lo + 15) / 16 * HD * 4; i += NW * 64) {
-                uint32_t* w = (uint32_t*)(a.c.v + at) + i;
+                uint32_t* w4 = (uint32_t*)(a.c.v + at) + i;
                 const int left = lo - (i / (HD * 4) * 16 + i % 4 * 4);  // of the word's four slots those before lo
                 if (left <= 0) continue;
-                const uint32_t mask = left >= 4 ? 0xffffffffu : (1u << 8 * left) - 1, o = *w;
-                *w = (e4m3_shift(o, vb - v_old) & mask) | (o & ~mask);
+                const uint32_t mask = left >= 4 ? 0xffffffffu : (1u << 8 * left) - 1, o = *w4;
+                *w4 = (e4m3_shift(o, vb - v_old) & mask) | (o & ~mask);
             }
     }
     const float kf = __uint_as_float((uint32_t)(254 - kb) << 23), vf = __uint_as_float((uint32_t)(254 - vb) << 23);
 #pragma unroll
-    for (int i = 0; i < APPEND_TOKENS; ++i) {
-        const int slot = lo + i * NW + wv;
+    for (int i = 0; i < APPEND_STEPS; ++i) {
+        const int slot = slot_of(i);
         if (slot >= hi) continue;
-        uint8_t* ko = a.c.k + at + (size_t)slot * HD + lane * E;
-        uint8_t* vo = codes + (i * NW + wv) * HD + lane * E;
-        if constexpr (E == 4) {
-            *(uint32_t*)ko = e4m3_byte(k[i][0] * kf) | e4m3_byte(k[i][1] * kf) << 8 | e4m3_byte(k[i][2] * kf) << 16 | e4m3_byte(k[i][3] * kf) << 24;
-            *(uint32_t*)vo = e4m3_byte(v[i][0] * vf) | e4m3_byte(v[i][1] * vf) << 8 | e4m3_byte(v[i][2] * vf) << 16 | e4m3_byte(v[i][3] * vf) << 24;
-        } else if constexpr (E == 2) {
-            *(uint16_t*)ko = (uint16_t)(e4m3_byte(k[i][0] * kf) | e4m3_byte(k[i][1] * kf) << 8);
-            *(uint16_t*)vo = (uint16_t)(e4m3_byte(v[i][0] * vf) | e4m3_byte(v[i][1] * vf) << 8);
-        } else {
-            *ko = (uint8_t)e4m3_byte(k[i][0] * kf);
-            *vo = (uint8_t)e4m3_byte(v[i][0] * vf);
-        }
+        uint8_t *ko = a.c.k + at + (size_t)slot * HD, *vo = codes + (slot - lo) * HD;
+        float v[8];
+        widen_dims(w[i][2], w[i][3], v);
+        *(uint32_t*)(ko + l.lo) = e4m3_four(k[i][0] * kf, k[i][1] * kf, k[i][2] * kf, k[i][3] * kf);
+        *(uint32_t*)(ko + l.hi) = e4m3_four(k[i][4] * kf, k[i][5] * kf, k[i][6] * kf, k[i][7] * kf);
+        *(uint32_t*)(vo + l.lo) = e4m3_four(v[0] * vf, v[1] * vf, v[2] * vf, v[3] * vf);
+        *(uint32_t*)(vo + l.hi) = e4m3_four(v[4] * vf, v[5] * vf, v[6] * vf, v[7] * vf);
     }
     __syncthreads();  // also: the page's words coded again are written before new bytes go into them
     // Values: a thread takes a dim of a group of sixteen slots.
@@ -207,14 +242,14 @@ __global__ __launch_bounds__(NW * 64) void paged_append_kernel(const PagedAppend
         const int s0 = max(lo, g * 16), s1 = min(hi, g * 16 + 16);
         const uint8_t* from = codes + d;
         if (s1 - s0 == 16) {
-            uint32_t w[4];
+            uint32_t w4[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                w[j] = 0;
+                w4[j] = 0;
 #pragma unroll
-                for (int b = 0; b < 4; ++b) w[j] |= (uint32_t)from[(s0 - lo + j * 4 + b) * HD] << 8 * b;
+                for (int b = 0; b < 4; ++b) w4[j] |= (uint32_t)from[(s0 - lo + j * 4 + b) * HD] << 8 * b;
             }
-            *(uint4*)vo = make_uint4(w[0], w[1], w[2], w[3]);
+            *(uint4*)vo = make_uint4(w4[0], w4[1], w4[2], w4[3]);
         } else {
             for (int s = s0; s < s1; ++s) vo[s - g * 16] = from[(s - lo) * HD];
         }
@@ -229,24 +264,23 @@ hipError_t q38_paged_append(const PagedAppendArgs& a0, hipStream_t stream) {
     PagedAppendArgs a = a0;
     const int ps = a.c.page_size;
     a.visits = (a.r.max_tokens + ps - 2) / ps + 1;
-    // Four waves while a page's new tokens fit their registers, else sixteen.
-    const bool few = (a.r.max_tokens < ps ? a.r.max_tokens : ps) <= 4 * APPEND_TOKENS;
-    const int nw = few ? 4 : 16;
-    a.kv_blocks = a.r.rows * a.visits * a.c.kv_heads;
-    const int groups = (a.q_heads + APPEND_HEADS - 1) / APPEND_HEADS;
-    const int grid = a.kv_blocks + (a.q ? (int)(((size_t)a.r.tokens * groups + nw - 1) / nw) : 0);
-    if (!grid) return hipSuccess;
-#define APPEND(E)                                                                                                   \
+    // Four waves where a page's new tokens fit their registers, else sixteen.
+    const int hd = a.c.head_dim, most = a.r.max_tokens < ps ? a.r.max_tokens : ps, nw = most <= append_room(hd, 4) ? 4 : 16;
+    const long long kv = (long long)a.r.rows * a.visits * a.c.kv_heads, vectors = a.q ? (long long)a.r.tokens * a.q_heads : 0;
+    const long long grid = kv + (vectors + append_room(hd, nw) - 1) / append_room(hd, nw);
+    if (grid > 0x7fffffff) return hipErrorInvalidConfiguration;
+    a.kv_blocks = (int)kv;
+#define APPEND(HD)                                                                                                  \
     do {                                                                                                            \
-        if (few)                                                                                                    \
-            hipLaunchKernelGGL((paged_append_kernel<E, 4>), dim3(grid), dim3(256), 0, stream, a);                   \
+        if (nw == 4)                                                                                                  \
+            hipLaunchKernelGGL((paged_append_kernel<HD, 4>), dim3(grid), dim3(256), 0, stream, a);                   \
         else                                                                                                        \
-            hipLaunchKernelGGL((paged_append_kernel<E, 16>), dim3(grid), dim3(1024), 0, stream, a);                 \
+            hipLaunchKernelGGL((paged_append_kernel<HD, 16>), dim3(grid), dim3(1024), 0, stream, a);                 \
     } while (0)
     switch (a.c.head_dim) {
-        case 64: APPEND(1); break;
-        case 128: APPEND(2); break;
-        case 256: APPEND(4); break;
+        case 64: APPEND(64); break;
+        case 128: APPEND(128); break;
+        case 256: APPEND(256); break;
         default: return hipErrorInvalidValue;
     }
 #undef APPEND
