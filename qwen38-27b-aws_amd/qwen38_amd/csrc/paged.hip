@@ -101,31 +101,32 @@ __device__ __forceinline__ void load_gain(const bf16_t* w, const HeadLane& l, fl
     for (int e = 0; e < 8; ++e) gain[e] += 1.0f;
 }
 
-constexpr int APPEND_STEPS = 4;  // a lane's vectors of one page, or of the queries: all of them stay in its registers
+constexpr int QUERY_STEPS = 4;  // a lane's vectors of the queries
 
-// Tokens of one page that a workgroup of nw waves has room for.
-constexpr int append_room(int head_dim, int nw) { return nw * (64 / (head_dim / 8)) * APPEND_STEPS; }
+// Vectors that nw waves hold at `steps` to a lane: of a page all new ones, in their registers.
+constexpr int append_room(int head_dim, int nw, int steps) { return nw * (64 / (head_dim / 8)) * steps; }
 
 }  // namespace
 
-// Grid: per row, page it may touch and KV head one workgroup; then the queries, APPEND_STEPS vectors per lane. A workgroup has all
+// Grid: per row, page it may touch and KV head one workgroup; then the queries, QUERY_STEPS vectors per lane. A workgroup has all
 // of its page's new tokens, so the page's largest value is known before any of them is coded, and every input is read once.
 // Bound: memory; for a few tokens a launch's and two loads' time.
-template <int HD, int NW>
+template <int HD, int NW, int STEPS>
 __global__ __launch_bounds__(NW * 64) void paged_append_kernel(const PagedAppendArgs a) {
     constexpr int VECS = 64 / (HD / 8);  // vectors of a wave at a time
     __shared__ float amax[2][NW];
-    __shared__ __attribute__((aligned(16))) uint8_t codes[128 * HD];  // the new values, [token][dim]
+    constexpr int ROOM = append_room(HD, NW, STEPS);
+    __shared__ __attribute__((aligned(16))) uint8_t codes[(ROOM < 128 ? ROOM : 128) * HD];  // the new values, [token][dim]
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int Hkv = a.c.kv_heads, ps = a.c.page_size;
     const HeadLane l = head_lane<HD>(lane, a.rot);
     float gain[8];
     if ((int)blockIdx.x >= a.kv_blocks) {
         const long long tokens = a.r.q_start ? min(a.r.q_start[a.r.rows], a.r.tokens) : a.r.tokens;
-        const long long first = ((long long)(blockIdx.x - a.kv_blocks) * NW + wv) * (VECS * APPEND_STEPS) + l.vec;
-        words2 lo[APPEND_STEPS], hi[APPEND_STEPS];
+        const long long first = ((long long)((int)blockIdx.x - a.kv_blocks) * NW + wv) * (VECS * QUERY_STEPS) + l.vec;
+        words2 lo[QUERY_STEPS], hi[QUERY_STEPS];
 #pragma unroll
-        for (int i = 0; i < APPEND_STEPS; ++i) {
+        for (int i = 0; i < QUERY_STEPS; ++i) {
             const long long u = first + i * VECS;
             const int t = (int)(u / a.q_heads), h = (int)(u % a.q_heads);
             lo[i] = hi[i] = (words2){0, 0};
@@ -133,7 +134,7 @@ __global__ __launch_bounds__(NW * 64) void paged_append_kernel(const PagedAppend
         }
         load_gain(a.q_norm, l, gain);
 #pragma unroll
-        for (int i = 0; i < APPEND_STEPS; ++i) {
+        for (int i = 0; i < QUERY_STEPS; ++i) {
             const long long u = first + i * VECS;
             const int t = (int)(u / a.q_heads), at = min(t, a.r.tokens - 1);
             float x[8];
@@ -154,25 +155,24 @@ __global__ __launch_bounds__(NW * 64) void paged_append_kernel(const PagedAppend
     const int page = r.p0 / ps + y, base = page * ps;
     const int lo = max(r.p0 - base, 0), hi = min(r.p0 + r.n - base, ps);  // the new tokens' slots
     if (lo >= hi) return;
-    const int id = paged_find(a.r, a.r.pages + (size_t)row * a.r.max_pages, page, a.c.pages);
-    if (id < 0) return;
-    const size_t head = (size_t)id * Hkv + kvh, at = head * ps * HD;
-    const int k_old = a.c.k_scale[head], v_old = a.c.v_scale[head];
-
-    float k[APPEND_STEPS][8], km = 0.0f, vm = 0.0f;
-    words2 w[APPEND_STEPS][4];  // the new keys and values
+    float k[STEPS][8], km = 0.0f, vm = 0.0f;
+    words2 w[STEPS][4];  // the new keys and values
     const int t0 = r.t0 + base - r.p0;  // the token of slot 0
     auto slot_of = [&](int i) { return lo + (i * NW + wv) * VECS + l.vec; };
 #pragma unroll
-    for (int i = 0; i < APPEND_STEPS; ++i) {
+    for (int i = 0; i < STEPS; ++i) {
         if (lo + (i * NW + wv) * VECS >= hi) continue;
         const size_t t = t0 + min(slot_of(i), hi - 1);
         load_dims(a.k + t * a.k_token + kvh * a.k_head, l, w[i][0], w[i][1]);
         load_dims(a.v + t * a.v_token + kvh * a.v_head, l, w[i][2], w[i][3]);
     }
+    const int id = paged_find(a.r, a.r.pages + (size_t)row * a.r.max_pages, page, a.c.pages);
+    if (id < 0) return;
+    const size_t head = (size_t)id * Hkv + kvh, at = head * ps * HD;
+    const int k_old = a.c.k_scale[head], v_old = a.c.v_scale[head];
     load_gain(a.k_norm, l, gain);
 #pragma unroll
-    for (int i = 0; i < APPEND_STEPS; ++i) {
+    for (int i = 0; i < STEPS; ++i) {
         if (lo + (i * NW + wv) * VECS >= hi) continue;
         const size_t t = t0 + min(slot_of(i), hi - 1);  // past the last token: that one again
         widen_dims(w[i][0], w[i][1], k[i]);
@@ -223,7 +223,7 @@ __global__ __launch_bounds__(NW * 64) void paged_append_kernel(const PagedAppend
     }
     const float kf = __uint_as_float((uint32_t)(254 - kb) << 23), vf = __uint_as_float((uint32_t)(254 - vb) << 23);
 #pragma unroll
-    for (int i = 0; i < APPEND_STEPS; ++i) {
+    for (int i = 0; i < STEPS; ++i) {
         const int slot = slot_of(i);
         if (slot >= hi) continue;
         uint8_t *ko = a.c.k + at + (size_t)slot * HD, *vo = codes + (slot - lo) * HD;
@@ -264,18 +264,25 @@ hipError_t q38_paged_append(const PagedAppendArgs& a0, hipStream_t stream) {
     PagedAppendArgs a = a0;
     const int ps = a.c.page_size;
     a.visits = (a.r.max_tokens + ps - 2) / ps + 1;
-    // Four waves where a page's new tokens fit their registers, else sixteen.
-    const int hd = a.c.head_dim, most = a.r.max_tokens < ps ? a.r.max_tokens : ps, nw = most <= append_room(hd, 4) ? 4 : 16;
+    // The fewest waves and registers that have room for a page's new tokens: a workgroup's time is a few loads', one after
+    // another, and with one vector per lane eight workgroups share a CU (37 ragged prompts in pages of 16).
+    const int hd = a.c.head_dim, most = a.r.max_tokens < ps ? a.r.max_tokens : ps;
+    const int nw = most <= append_room(hd, 4, 4) ? 4 : 16, steps = most <= append_room(hd, 4, 1) ? 1 : most <= append_room(hd, 4, 4) ? 4 : most <= append_room(hd, 16, 2) ? 2 : 4;
     const long long kv = (long long)a.r.rows * a.visits * a.c.kv_heads, vectors = a.q ? (long long)a.r.tokens * a.q_heads : 0;
-    const long long grid = kv + (vectors + append_room(hd, nw) - 1) / append_room(hd, nw);
+    const long long grid = kv + (vectors + append_room(hd, nw, QUERY_STEPS) - 1) / append_room(hd, nw, QUERY_STEPS);
     if (grid > 0x7fffffff) return hipErrorInvalidConfiguration;
     a.kv_blocks = (int)kv;
-#define APPEND(HD)                                                                                                  \
-    do {                                                                                                            \
-        if (nw == 4)                                                                                                  \
-            hipLaunchKernelGGL((paged_append_kernel<HD, 4>), dim3(grid), dim3(256), 0, stream, a);                   \
-        else                                                                                                        \
-            hipLaunchKernelGGL((paged_append_kernel<HD, 16>), dim3(grid), dim3(1024), 0, stream, a);                 \
+#define APPEND1(HD, NW, STEPS) hipLaunchKernelGGL((paged_append_kernel<HD, NW, STEPS>), dim3(grid), dim3(NW * 64), 0, stream, a)
+#define APPEND(HD)                \
+    do {                          \
+        if (nw == 4 && steps == 1) \
+            APPEND1(HD, 4, 1);    \
+        else if (nw == 4)         \
+            APPEND1(HD, 4, 4);    \
+        else if (steps == 2)      \
+            APPEND1(HD, 16, 2);   \
+        else                      \
+            APPEND1(HD, 16, 4);   \
     } while (0)
     switch (a.c.head_dim) {
         case 64: APPEND(64); break;
@@ -284,6 +291,7 @@ hipError_t q38_paged_append(const PagedAppendArgs& a0, hipStream_t stream) {
         default: return hipErrorInvalidValue;
     }
 #undef APPEND
+#undef APPEND1
     return hipGetLastError();
 }
 
