@@ -399,17 +399,17 @@ class _QueryArgs(ctypes.Structure):
                 ("cap", ctypes.c_float), ("window", ctypes.c_int), ("slopes", ctypes.c_void_p), ("prefix", ctypes.c_void_p)]
 
 
-def _want(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, device: torch.device) -> int:
-    """The device pointer of a contiguous tensor of this type, shape and device; ValueError if it is another."""
-    if t.dtype is not dtype or t.shape != shape or t.device != device:
-        raise ValueError(f"{name} must be {dtype} {list(shape)} on {device}, got {t.dtype} {list(t.shape)} on {t.device}")
-    return ptr(t)
+def _want(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, device: int) -> int:
+    """The pointer of a contiguous tensor of this type and shape on this device (its index); ValueError if it is another."""
+    if t.dtype is dtype and t.shape == shape and t.get_device() == device and t.is_contiguous():
+        return t.data_ptr()
+    raise ValueError(f"{name} must be contiguous {dtype} {list(shape)} on device {device}, got {t.dtype} {list(t.shape)} on {t.device}")
 
 
-def _heads_of(name: str, t: torch.Tensor, tokens: int | None, head_dim: int, device: torch.device) -> tuple[int, int, int]:
+def _heads_of(name: str, t: torch.Tensor, tokens: int, head_dim: int, device: int) -> tuple[int, int, int]:
     """Pointer and token and head strides of bf16 [tokens, heads, head_dim] whose last dim is contiguous."""
-    if t.dtype is not torch.bfloat16 or t.dim() != 3 or t.shape[2] != head_dim or t.device != device or (tokens is not None and t.shape[0] != tokens):
-        raise ValueError(f"{name} must be torch.bfloat16 [{'tokens' if tokens is None else tokens}, heads, {head_dim}] on {device}, got {t.dtype} {list(t.shape)} on {t.device}")
+    if t.dtype is not torch.bfloat16 or t.dim() != 3 or t.shape[0] != tokens or t.shape[2] != head_dim or t.get_device() != device:
+        raise ValueError(f"{name} must be torch.bfloat16 [{tokens}, heads, {head_dim}] on device {device}, got {t.dtype} {list(t.shape)} on {t.device}")
     token, head, one = t.stride()
     if one != 1:
         raise ValueError(f"{name}'s last dim must be contiguous")
@@ -417,12 +417,12 @@ def _heads_of(name: str, t: torch.Tensor, tokens: int | None, head_dim: int, dev
 
 
 def _paged_args(cache: PagedCache, position: torch.Tensor, pages: torch.Tensor, tokens: int, q_start, max_tokens):
-    """The cache and the rows of a call as the library takes them."""
-    k, device = cache.k, cache.k.device
+    """The cache and the rows of a call as the library takes them, and the index of their device."""
+    k = cache.k
     if not k.is_cuda or k.dim() != 4:
         raise ValueError("the cache must be on a device, its keys [pages, kv_heads, page, head_dim]")
+    device, u8, i32 = k.get_device(), torch.uint8, torch.int32
     count, heads, size, hd = k.shape
-    u8 = torch.uint8
     c = _CacheArgs(_want("cache.k", k, u8, (count, heads, size, hd), device), _want("cache.v", cache.v, u8, (count, heads, size // 16, hd, 16), device),
                    _want("cache.k_scale", cache.k_scale, u8, (count, heads), device),
                    _want("cache.v_scale", cache.v_scale, u8, (count, heads), device), count, heads, hd, size)
@@ -432,22 +432,22 @@ def _paged_args(cache: PagedCache, position: torch.Tensor, pages: torch.Tensor, 
     if q_start is None:
         if rows < 1 or tokens % rows:
             raise ValueError(f"{tokens} tokens are not the same number in each of {rows} rows: say where they start (q_start)")
-        max_tokens = tokens // rows
+        start, max_tokens = None, tokens // rows
     elif max_tokens is None:
         raise ValueError("ragged rows (q_start) need max_tokens, the most tokens of a row")
-    i32 = torch.int32
-    r = _RowArgs(_want("position", position, i32, (rows,), device), _want("pages", pages, i32, (rows, width), device),
-                 None if q_start is None else _want("q_start", q_start, i32, (rows + 1,), device), rows, width, tokens, min(max_tokens, tokens))
-    return c, r, device
-
-
-def _paged_call(device: torch.device, call) -> None:
-    """call(stream) on the device's current stream."""
-    if device.index == torch.cuda.current_device():
-        check(call(stream()))
     else:
+        start, max_tokens = _want("q_start", q_start, i32, (rows + 1,), device), min(max_tokens, tokens)
+    return c, _RowArgs(_want("position", position, i32, (rows,), device), _want("pages", pages, i32, (rows, width), device), start, rows, width,
+                       tokens, max_tokens), device
+
+
+def _on(device: int, fn, *args) -> None:
+    """fn(*args, stream) with the device's current stream (its number as torch's own code asks for it: `stream` takes longer than
+    the rest of a small call's checks)."""
+    if device != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
-            check(call(stream()))
+            return _on(device, fn, *args)
+    check(fn(*args, torch._C._cuda_getCurrentRawStream(device)))
 
 
 def paged_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, position: torch.Tensor, pages: torch.Tensor, *, cos=None, sin=None,
@@ -457,36 +457,36 @@ def paged_append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, position: 
     row's first new position (negative: the row is skipped), pages int32 [rows, max_pages] its page table, q_start int32 [rows + 1]
     where its tokens start (None: the same number in each row; else max_tokens is the most that a row has). With queries q
     [tokens, q_heads, hd] they are normed and rotated beside the keys and returned (in q_out, or a new tensor)."""
-    tokens = k.shape[0]
+    tokens, bf = k.shape[0], torch.bfloat16
     c, r, device = _paged_args(cache, position, pages, tokens, q_start, max_tokens)
-    t = _TokenArgs()
-    t.k, t.k_token, t.k_head = _heads_of("k", k, None, c.head_dim, device)
-    t.v, t.v_token, t.v_head = _heads_of("v", v, tokens, c.head_dim, device)
+    hd, rot = c.head_dim, 0
+    kp, k_token, k_head = _heads_of("k", k, tokens, hd, device)
+    vp, v_token, v_head = _heads_of("v", v, tokens, hd, device)
     if k.shape[1] != c.kv_heads or v.shape[1] != c.kv_heads:
         raise ValueError(f"keys and values of {c.kv_heads} heads, got {k.shape[1]} and {v.shape[1]}")
-    bf = torch.bfloat16
-    if (cos is None) != (sin is None):
-        raise ValueError("cos and sin go together")
-    if cos is not None:
-        if cos.dim() != 2:
-            raise ValueError(f"cos must be [tokens, rotary_dim], got {list(cos.shape)}")
-        t.rotary_dim = cos.shape[1]
-        t.cos, t.sin = _want("cos", cos, bf, (tokens, t.rotary_dim), device), _want("sin", sin, bf, (tokens, t.rotary_dim), device)
-    if k_norm is not None:
-        t.k_norm = _want("k_norm", k_norm, bf, (c.head_dim,), device)
-    if q is not None:
-        t.q, t.q_token, t.q_head = _heads_of("q", q, tokens, c.head_dim, device)
-        t.q_heads = q.shape[1]
-        if q_norm is not None:
-            t.q_norm = _want("q_norm", q_norm, bf, (c.head_dim,), device)
+    if cos is None:
+        if sin is not None:
+            raise ValueError("cos and sin go together")
+        cp = sp = None
+    else:
+        if sin is None or cos.dim() != 2:
+            raise ValueError("cos and sin go together, [tokens, rotary_dim]")
+        rot = cos.shape[1]
+        cp, sp = _want("cos", cos, bf, (tokens, rot), device), _want("sin", sin, bf, (tokens, rot), device)
+    kn = None if k_norm is None else _want("k_norm", k_norm, bf, (hd,), device)
+    if q is None:
+        if q_norm is not None or q_out is not None:
+            raise ValueError("q_norm and q_out need q")
+        t = _TokenArgs(kp, vp, None, None, k_token, k_head, v_token, v_head, 0, 0, 0, rot, cp, sp, None, kn, eps)
+    else:
+        qp, q_token, q_head = _heads_of("q", q, tokens, hd, device)
+        heads = q.shape[1]
         if q_out is None:
-            q_out = torch.empty(tokens, t.q_heads, c.head_dim, dtype=bf, device=device)
-        t.q_out = _want("q_out", q_out, bf, (tokens, t.q_heads, c.head_dim), device)
-    elif q_norm is not None or q_out is not None:
-        raise ValueError("q_norm and q_out need q")
-    t.eps = eps
+            q_out = torch.empty(tokens, heads, hd, dtype=bf, device=k.device)
+        t = _TokenArgs(kp, vp, qp, _want("q_out", q_out, bf, (tokens, heads, hd), device), k_token, k_head, v_token, v_head, q_token, q_head, heads,
+                       rot, cp, sp, None if q_norm is None else _want("q_norm", q_norm, bf, (hd,), device), kn, eps)
     ref = ctypes.byref
-    _paged_call(device, lambda s: library().q38_paged_append(ref(c), ref(r), ref(t), s))
+    _on(device, library().q38_paged_append, ref(c), ref(r), ref(t))
     return q_out
 
 
@@ -500,19 +500,18 @@ def paged_attention(cache: PagedCache, q: torch.Tensor, position: torch.Tensor, 
         raise ValueError(f"q must be [tokens, q_heads, hd], got {list(q.shape)}")
     tokens, heads, hd = q.shape
     c, r, device = _paged_args(cache, position, pages, tokens, q_start, max_tokens)
-    shape = (tokens, heads, c.head_dim)
-    qp = _want("q", q, torch.bfloat16, shape, device)
+    bf, shape = torch.bfloat16, (tokens, heads, c.head_dim)
+    qp = _want("q", q, bf, shape, device)
     if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=device)
-    a = _QueryArgs(qp, _want("out", out, torch.bfloat16, shape, device), heads, hd**-0.5 if scale is None else scale, cap, window)
-    if slopes is not None:
-        a.slopes = _want("slopes", slopes, torch.float32, (heads,), device)
-    if prefix is not None:
-        a.prefix = _want("prefix", prefix, torch.int32, (r.rows,), device)
+        out = torch.empty(shape, dtype=bf, device=q.device)
+    a = _QueryArgs(qp, _want("out", out, bf, shape, device), heads, hd**-0.5 if scale is None else scale, cap, window,
+                   None if slopes is None else _want("slopes", slopes, torch.float32, (heads,), device),
+                   None if prefix is None else _want("prefix", prefix, torch.int32, (r.rows,), device))
     ref, lib = ctypes.byref, library()
-    need = lib.q38_paged_attention_scratch(ref(c), ref(r), heads)
-    if scratch is None and need:
-        scratch = torch.empty(need, dtype=torch.uint8, device=device)
-    size = 0 if scratch is None else scratch.numel() * scratch.element_size()
-    _paged_call(device, lambda s: lib.q38_paged_attention(ref(c), ref(r), ref(a), ptr(scratch), size, s))
+    if scratch is None:
+        size = lib.q38_paged_attention_scratch(ref(c), ref(r), heads)
+        scratch = torch.empty(size, dtype=torch.uint8, device=q.device)
+    else:
+        size = scratch.numel() * scratch.element_size()
+    _on(device, lib.q38_paged_attention, ref(c), ref(r), ref(a), _want("scratch", scratch, scratch.dtype, scratch.shape, device), size)
     return out

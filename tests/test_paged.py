@@ -85,14 +85,14 @@ def test_host_tensors_and_wrong_shapes_are_refused():
             call()
     with pytest.raises(ValueError, match="q must be"):
         ext.paged_attention(cache, x[0], i, i[None])
-    with pytest.raises(ValueError, match="must be torch.int32"):
-        ext._want("position", i.long(), torch.int32, (1,), torch.device("cpu"))
-    with pytest.raises(ValueError, match="must be torch.int32"):
-        ext._want("position", i, torch.int32, (2,), torch.device("cpu"))
+    with pytest.raises(ValueError, match="must be contiguous torch.int32"):
+        ext._want("position", i.long(), torch.int32, (1,), -1)
+    with pytest.raises(ValueError, match="must be contiguous torch.int32"):
+        ext._want("position", i, torch.int32, (2,), -1)
     with pytest.raises(ValueError, match="last dim"):
-        ext._heads_of("k", torch.zeros(1, 64, 64, dtype=torch.bfloat16).transpose(1, 2), 1, 64, torch.device("cpu"))
+        ext._heads_of("k", torch.zeros(1, 64, 64, dtype=torch.bfloat16).transpose(1, 2), 1, 64, -1)
     with pytest.raises(ValueError, match="k must be"):
-        ext._heads_of("k", x.float(), 1, 64, torch.device("cpu"))
+        ext._heads_of("k", x.float(), 1, 64, -1)
 
 
 def test_paged_values_reads_what_the_oracle_reads():
