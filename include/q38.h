@@ -76,6 +76,9 @@ typedef struct q38_config {
                             MFMA, each 64-input block summed to about 2^-15.5 of its sum |x w|; Q38_MFMA_BF16: both widened
                             exactly to bf16 for the bf16 MFMA (float32-grade sums, twice the MFMA time). The head's
                             group maxima always run on the bf16 MFMA (bf16 activations). */
+    int kv_pages;     /* 0: a slab of max_seq_len positions per row in every attention layer. Else each layer's caches are a
+                         q38_paged_cache of that many pages (below; kv_cache_format Q38_KV_FP8), the rows' pages in "page_table" */
+    int kv_page_size; /* positions of a page (16, 32, 64 or 128, a divisor of max_seq_len); read with kv_pages only */
 } q38_config;
 
 const char* q38_last_error(void);
@@ -105,7 +108,9 @@ void q38_destroy(q38_handle* h);
  *   linear_attn.pending_input bf16 [2][B][K][C]: two halves, the current one given by q38_parity
  *   self_attn.k_cache bf16 [B][Hkv][S][hd]; self_attn.v_cache bf16 [B][Hkv][S/32][hd][32] (transposed per 32 positions);
  *   with kv_cache_format FP8 the same layouts of e4m3 bytes, and self_attn.k_scale, self_attn.v_scale (bf16 [1], the
- *   checkpoint's static scales, reference checkpoint.py:227-233) among the layer's weights
+ *   checkpoint's static scales, reference checkpoint.py:227-233) among the layer's weights; with kv_pages self_attn.k_cache,
+ *   v_cache, k_scale, v_scale are the k, v, k_scale, v_scale of a q38_paged_cache, and page_table (model-wide, int32
+ *   [B][max_seq_len / kv_page_size]) names each row's pages, for every attention layer and the MTP layer alike
  *   with saved_states: linear_attn.saved_state bf16 [B][Hv][128][128], linear_attn.saved_conv bf16 [B][C][3]
  * Scratch: workspace (model-wide; its GEMM counters are zeroed when it is bound).
  * Optional, per decoder layer: probe, which a q38_verify call fills when it is bound (size from q38_buffer_size): as

@@ -17,6 +17,7 @@
 
 #include "../../../include/q38.h"
 #include "kernels.h"
+#include "paged.h"
 
 namespace {
 
@@ -95,6 +96,10 @@ struct q38_handle {
     // prefill scratch (with a prefill chunk in the config)
     size_t off_pqn = 0, off_pkn = 0, off_pv = 0, off_po = 0, off_pdecay = 0, off_ppt = 0, off_pqs = 0, off_pmx = 0, off_ppart = 0,
            off_prows = 0, off_pkw = 0, off_pvw = 0;
+    // paged caches (kv_pages in the config): a call's positions, its tokens' start and end and its row's pages (prefill), the
+    // rotated queries, the attention's outputs and its scratch
+    size_t off_pg_pos = 0, off_pg_start = 0, off_pg_row = 0, off_pg_q = 0, off_pg_o = 0, off_pg_scratch = 0, pg_scratch = 0;
+    int max_pages = 0;
     size_t part_floats;  // capacity of the split-K partial buffer
     int gate_groups;  // K ranges of the gated-delta gate projections
     int attn_nchunks;  // chunks of ATTN_CHUNK_MIN cached positions over S
@@ -192,6 +197,7 @@ size_t expected_size(const q38_handle* h, const std::string& name, int layer) {
         if (name == "head.probe") return (B * K + 31) / 32 * 32 * H * 2;
         if (name == "embed_tokens") return V * H * 2;
         if (name == "rope_table") return S * 2 * 64 * 2;
+        if (h->cfg.kv_pages && name == "page_table") return B * h->max_pages * 4;
         if (name == "workspace") return h->workspace_bytes;
         return 0;
     }
@@ -222,6 +228,10 @@ size_t expected_size(const q38_handle* h, const std::string& name, int layer) {
     if ((r = fp8("self_attn.o_proj", H, Hq * hd))) return r;
     if (name == "self_attn.q_norm" || name == "self_attn.k_norm") return hd * 2;
     const bool kv8 = h->cfg.kv_cache_format == Q38_KV_FP8;
+    if (h->cfg.kv_pages) {
+        if (name == "self_attn.k_cache" || name == "self_attn.v_cache") return (size_t)h->cfg.kv_pages * Hkv * h->cfg.kv_page_size * hd;
+        if (name == "self_attn.k_scale" || name == "self_attn.v_scale") return (size_t)h->cfg.kv_pages * Hkv;
+    }
     if (name == "self_attn.k_cache" || name == "self_attn.v_cache") return B * Hkv * S * hd * (kv8 ? 1 : 2);
     if (kv8 && (name == "self_attn.k_scale" || name == "self_attn.v_scale")) return 2;
     if (layer == h->cfg.num_layers) {
@@ -323,6 +333,82 @@ struct TokensScope {
         h->Tpad = Tpad;
     }
 };
+
+// The paged cache of layer `li`, and a call's rows: all of them, h->K tokens each, or a prefill chunk's one.
+PagedCache paged_cache(q38_handle* h, int li, bool* ok) {
+    return {get<uint8_t>(h, "self_attn.k_cache", li, ok), get<uint8_t>(h, "self_attn.v_cache", li, ok), get<uint8_t>(h, "self_attn.k_scale", li, ok),
+            get<uint8_t>(h, "self_attn.v_scale", li, ok), h->cfg.kv_pages, h->Hkv, h->hd, h->cfg.kv_page_size};
+}
+
+PagedRows paged_rows(q38_handle* h, bool chunk, bool* ok) {
+    const int32_t* pos = (const int32_t*)h->ws(h->off_pg_pos);
+    if (chunk) return {pos, (const int32_t*)h->ws(h->off_pg_row), (const int32_t*)h->ws(h->off_pg_start), 1, h->max_pages, h->T, h->T};
+    return {pos, get<int32_t>(h, "page_table", -1, ok), nullptr, h->B, h->max_pages, h->T, h->K};
+}
+
+// Before the layers of a call over paged caches: its rows' positions; a prefill chunk's row.
+int paged_begin(q38_handle* h, const int32_t* position, const float* active, hipStream_t stream) {
+    if (!h->cfg.kv_pages) return 0;
+    HIP_TRY(q38_paged_positions(position, active, h->B, (int*)h->ws(h->off_pg_pos), stream));
+    return 0;
+}
+
+int paged_begin_chunk(q38_handle* h, const int32_t* slot, const int32_t* start, const int32_t* n_valid, int tokens, hipStream_t stream) {
+    if (!h->cfg.kv_pages) return 0;
+    bool ok = true;
+    auto table = get<int32_t>(h, "page_table", -1, &ok);
+    if (!ok) return 1;
+    HIP_TRY(q38_paged_slot(slot, start, n_valid, tokens, h->B, h->S, table, h->max_pages, (int*)h->ws(h->off_pg_pos), (int*)h->ws(h->off_pg_start),
+                           (int*)h->ws(h->off_pg_row), stream));
+    return 0;
+}
+
+// The step's keys and values (from column kv_col of qkv [T][ld], per head side by side) into layer `li`'s pages; the queries of a
+// q|gate|k|v projection rotated into the workspace unless q_norm is null.
+int paged_append(q38_handle* h, int li, const PagedRows& rows, const uint16_t* qkv, int ld, int kv_col, const uint16_t* q_norm, const uint16_t* k_norm,
+                 const uint16_t* cos, const uint16_t* sin, hipStream_t stream) {
+    bool ok = true;
+    PagedAppendArgs a{};
+    a.c = paged_cache(h, li, &ok);
+    if (!ok) return 1;
+    a.r = rows;
+    a.k = qkv + kv_col;
+    a.v = a.k + (size_t)h->Hkv * h->hd;
+    a.k_token = a.v_token = a.q_token = ld;
+    a.k_head = a.v_head = h->hd;
+    a.q_head = 2 * h->hd;
+    if (q_norm) {
+        a.q = qkv;
+        a.q_out = (uint16_t*)h->ws(h->off_pg_q);
+        a.q_heads = h->Hq;
+    }
+    a.cos = cos;
+    a.sin = sin;
+    a.rot = h->cfg.rotary_dim;
+    a.q_norm = q_norm;
+    a.k_norm = k_norm;
+    a.eps = h->cfg.rms_norm_eps;
+    HIP_TRY(q38_paged_append(a, stream));
+    return 0;
+}
+
+int paged_attention(q38_handle* h, int li, const PagedRows& rows, const uint16_t* qkv, int ld, uint8_t* act, hipStream_t stream) {
+    bool ok = true;
+    PagedAttnArgs a{};
+    a.c = paged_cache(h, li, &ok);
+    if (!ok) return 1;
+    a.r = rows;
+    a.q = (const uint16_t*)h->ws(h->off_pg_q);
+    a.out = (uint16_t*)h->ws(h->off_pg_o);
+    a.q_heads = h->Hq;
+    a.scale = 0.0625f;  // 256 ** -0.5
+    a.plan = paged_attention_plan(a.c, a.r, h->Hq);
+    a.scratch = h->ws(h->off_pg_scratch);
+    if (a.plan.bytes > h->pg_scratch) return fail("the paged attention's scratch is too small");
+    HIP_TRY(q38_paged_attention(a, stream));
+    HIP_TRY(q38_paged_gate(a.out, qkv, ld, h->T, h->Hq, rows.q_start, act, stream));
+    return 0;
+}
 
 // Mixer of layer `li` on act_h; leaves x += mixer and act_h = e5m2(post_attention_layernorm(x)).
 int run_mixer(q38_handle* h, int li, const StepIO& io, int rd, int wr, hipStream_t stream) {
@@ -466,6 +552,7 @@ int run_mixer(q38_handle* h, int li, const StepIO& io, int rd, int wr, hipStream
         auto kn = get<uint16_t>(h, "self_attn.k_norm", li, &ok);
         auto kc = get<uint16_t>(h, "self_attn.k_cache", li, &ok);
         auto vc = get<uint16_t>(h, "self_attn.v_cache", li, &ok);
+        const PagedRows rows = h->cfg.kv_pages ? paged_rows(h, io.slot != nullptr, &ok) : PagedRows{};
         const bool kv8 = h->cfg.kv_cache_format == Q38_KV_FP8;
         const uint16_t* ks = kv8 ? get<uint16_t>(h, "self_attn.k_scale", li, &ok) : nullptr;
         const uint16_t* vs = kv8 ? get<uint16_t>(h, "self_attn.v_scale", li, &ok) : nullptr;
@@ -477,6 +564,12 @@ int run_mixer(q38_handle* h, int li, const StepIO& io, int rd, int wr, hipStream
         if (gemm(h, li, qkv_t, qkv_s, act_h, H, nqkv, EPI_BF16, qkv, nqkv, nqkv, nullptr, 0, stream)) return 1;
         if (probe && !io.decode && !io.slot)
             HIP_TRY(hipMemcpyAsync(probe + (size_t)h->T * H, qkv, (size_t)h->T * nqkv * 2, hipMemcpyDeviceToDevice, stream));
+        if (h->cfg.kv_pages) {
+            if (paged_append(h, li, rows, qkv, nqkv, h->Hq * h->hd * 2, qn, kn, io.cos, io.sin, stream)) return 1;
+            if (paged_attention(h, li, rows, qkv, nqkv, act_mid, stream)) return 1;
+            kmid = h->Hq * h->hd;
+            goto out_proj;
+        }
         if (io.slot) {
             PrefillAttnArgs p{};
             p.L = h->T;
@@ -664,6 +757,14 @@ int q38_create(const q38_config* cfg, q38_handle** out) {
     if (c.prefill_chunk < 0 || c.prefill_chunk % 32 || c.prefill_chunk > c.max_seq_len) bad += "prefill_chunk must be a multiple of 32 up to max_seq_len; ";
     if (c.weight_format != Q38_WEIGHTS_E4M3 && c.weight_format != Q38_WEIGHTS_MXFP4) bad += "unknown weight_format; ";
     if (c.kv_cache_format != Q38_KV_BF16 && c.kv_cache_format != Q38_KV_FP8) bad += "unknown kv_cache_format; ";
+    if (c.kv_pages < 0) bad += "kv_pages must not be negative; ";
+    if (c.kv_pages > 0) {
+        if (c.kv_page_size != 16 && c.kv_page_size != 32 && c.kv_page_size != 64 && c.kv_page_size != 128)
+            bad += "kv_page_size must be 16, 32, 64 or 128; ";
+        else if (c.max_seq_len % c.kv_page_size)
+            bad += "max_seq_len must be a multiple of kv_page_size; ";
+        if (c.kv_cache_format != Q38_KV_FP8) bad += "paged caches need kv_cache_format Q38_KV_FP8; ";
+    }
     if (c.projection_mfma != Q38_MFMA_BF16 && c.projection_mfma != Q38_MFMA_FP8) bad += "unknown projection_mfma; ";
     for (int i = 0; i < c.num_layers && i < Q38_MAX_LAYERS; ++i)
         if (c.layer_types[i] != Q38_LINEAR && c.layer_types[i] != Q38_FULL) bad += "unknown layer type; ";
@@ -712,7 +813,8 @@ int q38_create(const q38_config* cfg, q38_handle** out) {
     h->gate_groups = 8;
     while (h->gate_groups > 1 && (h->H % (64 * h->gate_groups) || h->H / (64 * h->gate_groups) > 16)) h->gate_groups /= 2;
     h->off_gates = take((size_t)h->gate_groups * Tp * 2 * h->Hv * 4);
-    const size_t heads = (size_t)h->B * h->Hkv;
+    if (c.kv_pages) h->max_pages = h->S / c.kv_page_size;
+    const size_t heads = c.kv_pages ? 0 : (size_t)h->B * h->Hkv;  // of the slab caches' attention
     h->attn_nchunks = (h->S + ATTN_CHUNK_MIN - 1) / ATTN_CHUNK_MIN;
     h->off_scores = take(heads * ATTN_QMAX * h->S * 2);
     h->off_astats = take(heads * h->attn_nchunks * ATTN_QMAX * 2 * 4);
@@ -720,7 +822,7 @@ int q38_create(const q38_config* cfg, q38_handle** out) {
     h->off_akv = take(heads * 2 * ATTN_KMAX * 256 * 4);
     h->off_aq = take(heads * ATTN_QMAX * 256 * 2);
     // attn_pv's split sums: at most about two workgroups per CU of 64 query rows x 256 dims each.
-    h->attn_pv_floats = h->S > ATTN_CHUNK ? (size_t)2 * device_cus() * ATTN_QMAX * 256 : 0;
+    h->attn_pv_floats = heads && h->S > ATTN_CHUNK ? (size_t)2 * device_cus() * ATTN_QMAX * 256 : 0;
     h->off_apv = take(h->attn_pv_floats * 4);
     h->off_apr = take(heads * ATTN_QMAX * (2 + ATTN_KMAX) * 4);
     h->off_htiles = take(Tv * H * 2);
@@ -749,15 +851,33 @@ int q38_create(const q38_config* cfg, q38_handle** out) {
         h->off_po = take(Tc * h->Hv * h->dk * 2);
         h->off_ppt = take(Tc / PREFILL_GDN_CHUNK * h->Hv * 2 * PREFILL_GDN_CHUNK * PREFILL_GDN_CHUNK * 4);
         h->off_pdecay = take(Tc * h->Hv * 3 * 4);
-        h->off_pqs = take((size_t)h->Hq * Tc * 256 * 2);
-        h->off_pmx = take((size_t)h->Hq * prefill_blocks(Tc, h->S) * Tc * 4);
-        h->prefill_slots = prefill_slots(c.prefill_chunk, h->S, h->Hq, h->Hkv);
-        h->off_ppart = take(h->prefill_slots * 4 * 64 * 256 * 2);
-        h->off_prows = take(h->prefill_slots * 256 * 4);
-        if (c.kv_cache_format == Q38_KV_FP8) {
-            h->off_pkw = take((size_t)h->Hkv * h->S * 256 * 2);
-            h->off_pvw = take((size_t)h->Hkv * h->S * 256 * 2);
+        if (!c.kv_pages) {
+            h->off_pqs = take((size_t)h->Hq * Tc * 256 * 2);
+            h->off_pmx = take((size_t)h->Hq * prefill_blocks(Tc, h->S) * Tc * 4);
+            h->prefill_slots = prefill_slots(c.prefill_chunk, h->S, h->Hq, h->Hkv);
+            h->off_ppart = take(h->prefill_slots * 4 * 64 * 256 * 2);
+            h->off_prows = take(h->prefill_slots * 256 * 4);
+            if (c.kv_cache_format == Q38_KV_FP8) {
+                h->off_pkw = take((size_t)h->Hkv * h->S * 256 * 2);
+                h->off_pvw = take((size_t)h->Hkv * h->S * 256 * 2);
+            }
         }
+    }
+    if (c.kv_pages) {
+        const PagedCache cache{nullptr, nullptr, nullptr, nullptr, c.kv_pages, h->Hkv, h->hd, c.kv_page_size};
+        const int32_t* some = &h->cfg.num_layers;  // a q_start that is there
+        auto need = [&](int rows, int tokens, const int32_t* q_start) {
+            h->pg_scratch = std::max(h->pg_scratch, paged_attention_plan(cache, {nullptr, nullptr, q_start, rows, h->max_pages, rows * tokens, tokens}, h->Hq).bytes);
+        };
+        need(h->B, h->K, nullptr);
+        need(h->B, 1, nullptr);
+        for (int l = 32; l <= c.prefill_chunk; l += 32) need(1, l, some);
+        h->off_pg_pos = take((size_t)h->B * 4);
+        h->off_pg_start = take(8);
+        h->off_pg_row = take((size_t)h->max_pages * 4);
+        h->off_pg_q = take(Tp * h->Hq * 256 * 2);
+        h->off_pg_o = take(Tp * h->Hq * 256 * 2);
+        h->off_pg_scratch = take(h->pg_scratch);
     }
     h->workspace_bytes = o;
     *out = h;
@@ -936,6 +1056,7 @@ int q38_verify(q38_handle* h, const uint16_t* embeds, const uint16_t* cos, const
     uint16_t* hbf = is_linear(h, 0) ? (uint16_t*)h->ws(h->off_hbf) : nullptr;
     if (norm_rows(h, nullptr, 0, embeds, nullptr, x, in0, h->ws(h->off_act_h), h->H, 0, hbf, nullptr, stream)) return 1;
     StepIO io{cos, sin, position, active, accepted};
+    if (paged_begin(h, position, active, stream)) return 1;
     for (int li = 0; li < L; ++li) {
         if (run_mixer(h, li, io, rd, wr, stream)) return 1;
         if (run_mlp(h, li, li + 1 < L ? li + 1 : -1, out_hidden, false, stream)) return 1;
@@ -958,6 +1079,7 @@ int q38_decode(q38_handle* h, const uint16_t* embeds, const uint16_t* cos, const
     uint16_t* hbf = is_linear(h, 0) ? (uint16_t*)h->ws(h->off_hbf) : nullptr;
     if (norm_rows(h, nullptr, 0, embeds, nullptr, x, in0, h->ws(h->off_act_h), h->H, 0, hbf, nullptr, stream)) return 1;
     StepIO io{cos, sin, position, active, nullptr, true};
+    if (paged_begin(h, position, active, stream)) return 1;
     for (int li = 0; li < L; ++li) {
         if (run_mixer(h, li, io, rd, wr, stream)) return 1;
         if (run_mlp(h, li, li + 1 < L ? li + 1 : -1, out_hidden, false, stream)) return 1;
@@ -983,6 +1105,7 @@ int q38_prefill(q38_handle* h, const uint16_t* embeds, const uint16_t* cos, cons
     uint16_t* hbf = is_linear(h, 0) ? (uint16_t*)h->ws(h->off_hbf) : nullptr;
     if (norm_rows(h, nullptr, 0, embeds, nullptr, x, in0, h->ws(h->off_act_h), h->H, 0, hbf, nullptr, stream)) return 1;
     StepIO io{cos, sin, nullptr, nullptr, nullptr, false, slot, start, n_valid};
+    if (paged_begin_chunk(h, slot, start, n_valid, tokens, stream)) return 1;
     for (int li = 0; li < L; ++li) {
         if (run_mixer(h, li, io, rd, rd, stream)) return 1;
         if (run_mlp(h, li, li + 1 < L ? li + 1 : -1, out_hidden, false, stream)) return 1;
@@ -1036,6 +1159,12 @@ int q38_mtp_prefill(q38_handle* h, const uint16_t* hidden, const uint16_t* embed
     if (gemm(h, M, qkv_t + q_rows / 32 * kt * 2048, qkv_s + q_rows / 32 * kt * 64, act_h, H, nkv, EPI_BF16, kv, nkv, nkv, nullptr, 0,
              stream))
         return 1;
+    if (h->cfg.kv_pages) {
+        if (paged_begin_chunk(h, slot, start, nullptr, tokens, stream)) return 1;
+        if (paged_append(h, M, paged_rows(h, true, &ok), kv, nkv, 0, nullptr, kn, cos, sin, stream)) return 1;
+        if (out_x) HIP_TRY(hipMemcpyAsync(out_x, x, (size_t)H * 2, hipMemcpyDeviceToDevice, stream));
+        return 0;
+    }
     PrefillAttnArgs p{};
     p.L = h->T;
     p.rows = h->B;
@@ -1122,6 +1251,7 @@ int q38_mtp_step(q38_handle* h, const uint16_t* hidden, const uint16_t* embeds, 
     if (norm_rows(h, (const float*)h->ws(h->off_part), splits, nullptr, nullptr, x, in0, act_h, H, 0, nullptr, nullptr, stream))
         return 1;
     StepIO io{cos, sin, position, active, nullptr};
+    if (paged_begin(h, position, active, stream)) return 1;
     if (run_mixer(h, M, io, 0, 0, stream)) return 1;
     return run_mlp(h, M, -1, out, true, stream);
 }

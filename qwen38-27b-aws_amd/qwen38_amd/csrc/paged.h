@@ -80,4 +80,11 @@ __device__ __forceinline__ int paged_find(const PagedRows& a, const int* table, 
 }
 
 hipError_t q38_paged_append(const PagedAppendArgs& a, hipStream_t stream);
+// The engine's glue: a step's positions with -1 for rows that are not active; a prefill call's one row (its page numbers, its
+// position, where its n_valid (null: all) tokens start and end; the position -1 if the chunk does not fit or there is no such
+// row); and the attention's outputs, gated, as the o projection's e5m2 input tiles (tokens past q_start[1]: zeros).
+hipError_t q38_paged_positions(const int* position, const float* active, int rows, int* out, hipStream_t stream);
+hipError_t q38_paged_slot(const int* slot, const int* start, const int* n_valid, int tokens, int rows, int seq, const int* table, int max_pages,
+                          int* position, int* q_start, int* pages, hipStream_t stream);
+hipError_t q38_paged_gate(const bf16_t* o, const bf16_t* qkv, int ld, int tokens, int q_heads, const int* q_start, uint8_t* act, hipStream_t stream);
 hipError_t q38_paged_attention(const PagedAttnArgs& a, hipStream_t stream);

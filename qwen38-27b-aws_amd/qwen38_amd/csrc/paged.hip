@@ -295,6 +295,54 @@ hipError_t q38_paged_append(const PagedAppendArgs& a0, hipStream_t stream) {
     return hipGetLastError();
 }
 
+// ---- The engine's glue.
+__global__ void paged_positions_kernel(const int* position, const float* active, int rows, int* out) {
+    const int b = blockIdx.x * 256 + threadIdx.x;
+    if (b < rows) out[b] = active[b] > 0.5f ? position[b] : -1;
+}
+
+hipError_t q38_paged_positions(const int* position, const float* active, int rows, int* out, hipStream_t stream) {
+    hipLaunchKernelGGL(paged_positions_kernel, dim3((rows + 255) / 256), dim3(256), 0, stream, position, active, rows, out);
+    return hipGetLastError();
+}
+
+__global__ __launch_bounds__(256) void paged_slot_kernel(const int* slot, const int* start, const int* n_valid, int tokens, int rows, int seq, const int* table,
+                                                         int max_pages, int* position, int* q_start, int* pages) {
+    const int b = *slot, p = *start;
+    const bool row = b >= 0 && b < rows;
+    if (threadIdx.x == 0) {
+        *position = row && p >= 0 && p <= seq - tokens ? p : -1;
+        q_start[0] = 0;
+        q_start[1] = n_valid ? min(max(*n_valid, 0), tokens) : tokens;
+    }
+    for (int i = threadIdx.x; i < max_pages; i += 256) pages[i] = row ? table[(size_t)b * max_pages + i] : -1;
+}
+
+hipError_t q38_paged_slot(const int* slot, const int* start, const int* n_valid, int tokens, int rows, int seq, const int* table, int max_pages,
+                          int* position, int* q_start, int* pages, hipStream_t stream) {
+    hipLaunchKernelGGL(paged_slot_kernel, dim3(1), dim3(256), 0, stream, slot, start, n_valid, tokens, rows, seq, table, max_pages, position, q_start, pages);
+    return hipGetLastError();
+}
+
+// Four dims per thread: bf16(o) x bf16(sigmoid(gate)) in bf16, then e5m2 (reference model.py:637-638, as every projection input).
+__global__ __launch_bounds__(256) void paged_gate_kernel(const bf16_t* o, const bf16_t* qkv, int ld, int tokens, int q_heads, const int* q_start, uint8_t* act) {
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    const int t = (int)(i / (q_heads * 64)), x = (int)(i % (q_heads * 64)) * 4;
+    if (t >= tokens) return;
+    uint32_t r = 0;
+    if (!q_start || t < q_start[1]) {
+        const uint2 v = *(const uint2*)(o + (size_t)t * q_heads * 256 + x), g = *(const uint2*)(qkv + (size_t)t * ld + x / 256 * 512 + 256 + x % 256);
+        r = pk_e5m2(rbf(lo_bf(v.x) * rbf(sigmoidf_(lo_bf(g.x)))), rbf(hi_bf(v.x) * rbf(sigmoidf_(hi_bf(g.x)))),
+                    rbf(lo_bf(v.y) * rbf(sigmoidf_(lo_bf(g.y)))), rbf(hi_bf(v.y) * rbf(sigmoidf_(hi_bf(g.y)))));
+    }
+    *(uint32_t*)(act + act_offset(t, x, q_heads * 256)) = r;
+}
+
+hipError_t q38_paged_gate(const bf16_t* o, const bf16_t* qkv, int ld, int tokens, int q_heads, const int* q_start, uint8_t* act, hipStream_t stream) {
+    hipLaunchKernelGGL(paged_gate_kernel, dim3(((size_t)tokens * q_heads * 64 + 255) / 256), dim3(256), 0, stream, o, qkv, ld, tokens, q_heads, q_start, act);
+    return hipGetLastError();
+}
+
 // ---- The C ABI (include/q38.h).
 namespace {
 

@@ -36,6 +36,7 @@ class Q38Config(ctypes.Structure):
         ("batch_size", ctypes.c_int), ("verify_tokens", ctypes.c_int), ("max_seq_len", ctypes.c_int), ("mtp", ctypes.c_int),
         ("saved_states", ctypes.c_int), ("prefill_chunk", ctypes.c_int), ("weight_format", ctypes.c_int),
         ("kv_cache_format", ctypes.c_int), ("projection_mfma", ctypes.c_int),
+        ("kv_pages", ctypes.c_int), ("kv_page_size", ctypes.c_int),
     ]
 
 
@@ -124,7 +125,7 @@ def stream() -> int:
 
 def make_config(cfg: TextConfig, batch: int, tokens: int, max_seq_len: int, mtp: bool, saved_states: bool = False,
                 prefill_chunk: int = 0, weight_format: str = "e4m3", kv_cache_format: str = "bf16",
-                projection_mfma: str = "bf16") -> Q38Config:
+                projection_mfma: str = "bf16", kv_pages: int = 0, kv_page_size: int = 64) -> Q38Config:
     c = Q38Config()
     c.hidden_size, c.intermediate_size, c.vocab_size = cfg.hidden_size, cfg.intermediate_size, cfg.vocab_size
     if cfg.num_hidden_layers > MAX_LAYERS:
@@ -144,6 +145,7 @@ def make_config(cfg: TextConfig, batch: int, tokens: int, max_seq_len: int, mtp:
     c.weight_format = WEIGHT_FORMATS[weight_format]
     c.kv_cache_format = KV_CACHE_FORMATS[kv_cache_format]
     c.projection_mfma = PROJECTION_MFMA[projection_mfma]
+    c.kv_pages, c.kv_page_size = kv_pages, kv_page_size
     return c
 
 
@@ -151,10 +153,11 @@ class Handle:
     """One q38_handle: shapes fixed at creation, every buffer bound by the owner."""
 
     def __init__(self, cfg: TextConfig, batch: int, tokens: int, max_seq_len: int, mtp: bool, saved_states: bool = False,
-                 prefill_chunk: int = 0, weight_format: str = "e4m3", kv_cache_format: str = "bf16", projection_mfma: str = "bf16"):
+                 prefill_chunk: int = 0, weight_format: str = "e4m3", kv_cache_format: str = "bf16", projection_mfma: str = "bf16",
+                 kv_pages: int = 0, kv_page_size: int = 64):
         self.lib = library()
         self.c = make_config(cfg, batch, tokens, max_seq_len, mtp, saved_states, prefill_chunk, weight_format, kv_cache_format,
-                             projection_mfma)
+                             projection_mfma, kv_pages, kv_page_size)
         h = ctypes.c_void_p()
         check(self.lib.q38_create(ctypes.byref(self.c), ctypes.byref(h)))
         self.h = h

@@ -61,12 +61,13 @@ def load(model_dir: str | Path | None = None, *, cfg: TextConfig | None = None,
          weights: Iterable[tuple[str, object]] | None = None, batch_size: int = 1, max_seq_len: int = 4096,
          verify_tokens: int = 0, chunk: int | None = None, mtp: bool = False, head_batch: int | None = None,
          mtp_build: dict | None = None, weight_format: str = "mxfp4", kv_cache_format: str = "bf16",
-         saved_states: bool = False, log: Callable[[str], None] = _log) -> Loaded:
+         saved_states: bool = False, kv_pages: int = 0, kv_page_size: int = 64, log: Callable[[str], None] = _log) -> Loaded:
     """The model of ``model_dir`` (its config.json, its safetensors files through `checkpoint.model_weights`, its
     tokenizer.json if present), or ``cfg`` with ``weights`` as (name, value) pairs (`synth.model_specs` names), on the
     GPU. ``head_batch`` is the head's rows (default rows x tokens); ``mtp_build`` ({"batch_size", "mtp_tokens",
     "chunk"}) describes a separately built drafter to check against the blocks, as the reference checks its MTP
-    build's info."""
+    build's info. ``kv_pages`` pages of ``kv_page_size`` positions in place of a slab per row (with ``kv_cache_format`` "fp8"): an
+    8-bit cache that needs no scales from the checkpoint."""
     from . import checkpoint
     from .generate import ChipHead
     from .steps import Engine, HeadGraph, MTPStep, StepGraph, VerifyStep
@@ -89,9 +90,9 @@ def load(model_dir: str | Path | None = None, *, cfg: TextConfig | None = None,
     started = time.perf_counter()
     engine = Engine(cfg, batch_size, max(verify_tokens, 1), max_seq_len, mtp=mtp, saved_states=saved_states,
                     prefill_chunk=chunk or 0, weight_format="mxfp4" if weight_format == "mxfp4" else "e4m3",
-                    kv_cache_format=kv_cache_format)
+                    kv_cache_format=kv_cache_format, kv_pages=kv_pages, kv_page_size=kv_page_size)
     engine.load(weights)
-    if kv_cache_format == "fp8" and model_dir is not None:
+    if kv_cache_format == "fp8" and not kv_pages and model_dir is not None:
         for i, (k, v) in checkpoint.kv_scales(model_dir, cfg).items():
             engine.set_kv_scales(i, k, v)
     torch.cuda.synchronize()

@@ -43,7 +43,7 @@ class Engine:
 
     def __init__(self, cfg: TextConfig, batch_size: int, verify_tokens: int, max_seq_len: int, mtp: bool = True, device="cuda",
                  saved_states: bool = False, prefill_chunk: int = 0, weight_format: str = "e4m3", kv_cache_format: str = "bf16",
-                 projection_mfma: str = "bf16"):
+                 projection_mfma: str = "bf16", kv_pages: int = 0, kv_page_size: int = 64):
         if not torch.cuda.is_available():
             raise RuntimeError("the verify path runs on the GPU only")
         self.cfg, self.batch_size, self.verify_tokens, self.max_seq_len, self.mtp = cfg, batch_size, verify_tokens, max_seq_len, mtp
@@ -52,7 +52,8 @@ class Engine:
         self.device = torch.device(device)
         self.projection_mfma = projection_mfma
         self.handle = ext.Handle(cfg, batch_size, verify_tokens, max_seq_len, mtp, saved_states, prefill_chunk, weight_format,
-                                 kv_cache_format, projection_mfma)
+                                 kv_cache_format, projection_mfma, kv_pages, kv_page_size)
+        self.kv_pages, self.kv_page_size = kv_pages, kv_page_size
         kv_dtype = torch.uint8 if kv_cache_format == "fp8" else DTYPE
         self.buffers: dict[tuple[str, int], torch.Tensor] = {}
         self.mtp_layer = cfg.num_hidden_layers
@@ -69,11 +70,14 @@ class Engine:
                     self._bind_zeros("linear_attn.saved_state", i, DTYPE)
                     self._bind_zeros("linear_attn.saved_conv", i, DTYPE)
             else:
-                self._bind_zeros("self_attn.k_cache", i, kv_dtype)
-                self._bind_zeros("self_attn.v_cache", i, kv_dtype)
+                self._bind_kv(i, kv_dtype)
         if mtp:
-            self._bind_zeros("self_attn.k_cache", self.mtp_layer, kv_dtype)
-            self._bind_zeros("self_attn.v_cache", self.mtp_layer, kv_dtype)
+            self._bind_kv(self.mtp_layer, kv_dtype)
+        if kv_pages:
+            # Every row its own run of pages while there are enough; rows past them, none (`set_pages` names others).
+            each = max_seq_len // kv_page_size
+            own = torch.arange(batch_size * each, dtype=torch.int32).reshape(batch_size, each)
+            self.bind("page_table", -1, torch.where(own < kv_pages, own, -1))
         if verify_tokens >= 2:
             # cos/sin of every position, which the on-device speculative steps gather by the positions they compute.
             from .generate import rope_table
@@ -87,6 +91,13 @@ class Engine:
         size = torch.empty((), dtype=dtype).element_size()
         t = torch.zeros(nbytes // size, dtype=dtype, device=self.device)
         return self.bind(name, layer, t)
+
+    def _bind_kv(self, layer: int, dtype: torch.dtype) -> None:
+        self._bind_zeros("self_attn.k_cache", layer, dtype)
+        self._bind_zeros("self_attn.v_cache", layer, dtype)
+        if self.kv_pages:
+            self._bind_zeros("self_attn.k_scale", layer, torch.uint8)
+            self._bind_zeros("self_attn.v_scale", layer, torch.uint8)
 
     def bind(self, name: str, layer: int, t: torch.Tensor) -> torch.Tensor:
         t = t.to(self.device).contiguous()
@@ -242,8 +253,34 @@ class Engine:
         tiles = self.buffer("head.probe", -1)[: t32 * h]
         return tiles[tile_offsets(t32, h, tiles.device)].reshape(t32, h)[:rows]
 
+    def paged_cache(self, layer: int) -> ext.PagedCache:
+        """A paged engine's cache of an attention layer (the MTP layer's too), for `ext.paged_values` and the operators."""
+        if not self.kv_pages:
+            raise ValueError("this engine's caches are slabs (kv_pages is 0)")
+        n, h, p, d = self.kv_pages, self.cfg.num_key_value_heads, self.kv_page_size, self.cfg.head_dim
+        get = lambda name: self.buffer("self_attn." + name, layer)  # noqa: E731
+        return ext.PagedCache(get("k_cache").view(n, h, p, d), get("v_cache").view(n, h, p // 16, d, 16), get("k_scale").view(n, h),
+                              get("v_scale").view(n, h))
+
+    @property
+    def page_table(self) -> torch.Tensor:
+        """A paged engine's rows' pages, int32 [B, max_seq_len / kv_page_size] on the device; -1: none."""
+        if not self.kv_pages:
+            raise ValueError("this engine's caches are slabs (kv_pages is 0)")
+        return self.buffer("page_table", -1).view(self.batch_size, -1)
+
+    def set_pages(self, row: int, pages: Sequence[int]) -> None:
+        """Row ``row``'s pages in order of its positions (at most max_seq_len / kv_page_size; the places after them hold none). Rows may
+        share pages that none of them appends to: those of a common prefix."""
+        table = self.page_table
+        if not 0 <= row < table.shape[0] or len(pages) > table.shape[1] or any(not 0 <= p < self.kv_pages for p in pages):
+            raise ValueError(f"row {row} of {table.shape[0]} takes up to {table.shape[1]} pages out of {self.kv_pages}")
+        table[row] = torch.tensor([*pages, *[-1] * (table.shape[1] - len(pages))], dtype=torch.int32)
+
     def kv_cache(self, layer: int) -> tuple[torch.Tensor, torch.Tensor]:
         """(k_cache [B,Hkv,S,hd], v_cache stored transposed [B,Hkv,S/32,hd,32])."""
+        if self.kv_pages:
+            raise ValueError("this engine's caches are paged: paged_cache")
         cfg, b, s = self.cfg, self.batch_size, self.max_seq_len
         kc = self.buffer("self_attn.k_cache", layer).view(b, cfg.num_key_value_heads, s, cfg.head_dim)
         vc = self.buffer("self_attn.v_cache", layer).view(b, cfg.num_key_value_heads, s // 32, cfg.head_dim, 32)
@@ -251,7 +288,10 @@ class Engine:
 
     def set_kv_scales(self, layer: int, k_scale: torch.Tensor, v_scale: torch.Tensor) -> None:
         """An FP8 cache's static scales for one attention layer (the MTP layer included): bf16 ``[1]`` each, the
-        reference's ``self_attn.k_scale`` / ``v_scale`` (model.py:559-561, checkpoint.py:227-233)."""
+        reference's ``self_attn.k_scale`` / ``v_scale`` (model.py:559-561, checkpoint.py:227-233). A paged cache finds its own
+        scales and takes none."""
+        if self.kv_pages:
+            raise ValueError("a paged cache takes no static scales")
         self.bind("self_attn.k_scale", layer, k_scale.reshape(1).to(DTYPE))
         self.bind("self_attn.v_scale", layer, v_scale.reshape(1).to(DTYPE))
 

@@ -104,3 +104,22 @@ def test_paged_values_reads_what_the_oracle_reads():
         t.copy_(torch.randint(100, 140, t.shape, generator=g).to(torch.uint8))
     for a, b in zip(ext.paged_values(cache), po.values(cache)[:2]):
         assert torch.equal(a.double().isnan(), b.isnan()) and torch.equal(a.double().nan_to_num(), b.nan_to_num())
+
+
+def test_an_engine_sizes_its_paged_caches_and_refuses_others():
+    from qwen38_amd.config import tiny_config
+
+    cfg = tiny_config(1)  # layers 0-2 gated delta, 3 attention; MTP layer 4
+    hkv = cfg.num_key_value_heads
+    h = ext.Handle(cfg, 4, 4, 128, True, prefill_chunk=64, kv_cache_format="fp8", kv_pages=40, kv_page_size=32)
+    for layer in (3, 4):
+        assert h.buffer_size("self_attn.k_cache", layer) == h.buffer_size("self_attn.v_cache", layer) == 40 * hkv * 32 * 256
+        assert h.buffer_size("self_attn.k_scale", layer) == h.buffer_size("self_attn.v_scale", layer) == 40 * hkv
+    assert h.buffer_size("page_table", -1) == 4 * 4 * 4
+    with pytest.raises(RuntimeError, match="no buffer"):
+        ext.Handle(cfg, 4, 4, 128, True).buffer_size("page_table", -1)
+    for changes, message in (({"kv_pages": -1}, "negative"), ({"kv_page_size": 48}, "kv_page_size"), ({"kv_page_size": 256}, "kv_page_size"),
+                             ({"max_seq_len": 160, "kv_page_size": 128}, "multiple of kv_page_size"), ({"kv_cache_format": "bf16"}, "FP8")):
+        kw = {"max_seq_len": 128, "kv_cache_format": "fp8", "kv_pages": 8, "kv_page_size": 64, **changes}
+        with pytest.raises(RuntimeError, match=message):
+            ext.Handle(cfg, 4, 4, kw.pop("max_seq_len"), True, **kw)
