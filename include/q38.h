@@ -295,14 +295,14 @@ typedef struct q38_paged_cache {
  * are taken). position int32 [rows]: the first token's position in its row; negative skips the row (nothing is appended, its
  * outputs are zero). pages int32 [rows][max_pages]: the pages of each row's positions in order. An entry outside [0, pages), like
  * a position past the table, names no page: nothing is appended there, and a query that sees it answers NaN. Rows may share
- * pages that none of them appends to. */
+ * pages that none of them appends to. rows * kv_heads is below 2^18, rows * max_tokens at most 2^24. */
 typedef struct q38_paged_rows {
     const int32_t *position, *pages, *q_start;
     int rows, max_pages, tokens, max_tokens;
 } q38_paged_rows;
 
 /* The tokens to append: keys, values and optionally queries (q null: none), bf16, token t's head h at t * *_token + h * *_head
- * elements (multiples of 4; the pointers 8-byte aligned), its head_dim elements side by side. Queries and keys are RMS-normed
+ * elements (multiples of 4; all pointers 8-byte aligned), its head_dim elements side by side. Queries and keys are RMS-normed
  * per head where q_norm, k_norm (bf16 [head_dim], used as 1 + w; null: no norm) say so, then their first rotary_dim dims (a
  * multiple of 8 up to head_dim; 0: no rotation) are rotated, d with d + rotary_dim / 2, by cos, sin bf16 [tokens][rotary_dim]; all
  * in float32. q_out bf16 [tokens][q_heads][head_dim] receives the queries, of the tokens of every row. */

@@ -88,3 +88,4 @@ hipError_t q38_paged_slot(const int* slot, const int* start, const int* n_valid,
                           int* position, int* q_start, int* pages, hipStream_t stream);
 hipError_t q38_paged_gate(const bf16_t* o, const bf16_t* qkv, int ld, int tokens, int q_heads, const int* q_start, uint8_t* act, hipStream_t stream);
 hipError_t q38_paged_attention(const PagedAttnArgs& a, hipStream_t stream);
+bool paged_attention_fits(const PagedCache& c, const PagedRows& r, int q_heads);

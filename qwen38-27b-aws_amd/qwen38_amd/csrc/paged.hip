@@ -270,7 +270,7 @@ hipError_t q38_paged_append(const PagedAppendArgs& a0, hipStream_t stream) {
     const int nw = most <= append_room(hd, 4, 4) ? 4 : 16, steps = most <= append_room(hd, 4, 1) ? 1 : most <= append_room(hd, 4, 4) ? 4 : most <= append_room(hd, 16, 2) ? 2 : 4;
     const long long kv = (long long)a.r.rows * a.visits * a.c.kv_heads, vectors = a.q ? (long long)a.r.tokens * a.q_heads : 0;
     const long long grid = kv + (vectors + append_room(hd, nw, QUERY_STEPS) - 1) / append_room(hd, nw, QUERY_STEPS);
-    if (grid > 0x7fffffff) return hipErrorInvalidConfiguration;
+    if (grid * nw * 64 > 0xffffffffLL) return hipErrorInvalidConfiguration;  // a grid's threads are counted in 32 bits
     a.kv_blocks = (int)kv;
 #define APPEND1(HD, NW, STEPS) hipLaunchKernelGGL((paged_append_kernel<HD, NW, STEPS>), dim3(grid), dim3(NW * 64), 0, stream, a)
 #define APPEND(HD)                \
@@ -358,6 +358,7 @@ const char* paged_bad(const q38_paged_cache* c, const q38_paged_rows* r) {
     if (r->max_tokens > r->tokens) return "paged rows: max_tokens above tokens";
     if (!r->q_start && (long long)r->rows * r->max_tokens != r->tokens) return "paged rows: without q_start tokens must be rows * max_tokens";
     if ((long long)r->max_pages * c->page_size > (1 << 30)) return "paged rows: more than 2^30 positions";
+    if ((long long)r->rows * c->kv_heads >= 1 << 18) return "paged rows: rows * kv_heads too large for one call";
     if ((long long)r->rows * (r->max_tokens + 2) > (1 << 24) || (long long)r->rows * r->max_tokens * c->kv_heads > (1 << 28))
         return "paged rows: rows * max_tokens too large for one call";
     return nullptr;
@@ -378,6 +379,8 @@ int q38_paged_append(const q38_paged_cache* c, const q38_paged_rows* r, const q3
         return q38_report("paged append: strides must be multiples of 4 elements");
     if ((uintptr_t)t->k % 8 || (uintptr_t)t->v % 8 || (uintptr_t)t->q % 8 || (uintptr_t)t->q_out % 8)
         return q38_report("paged append: keys, values and queries must be 8-byte aligned");
+    if ((uintptr_t)t->q_norm % 8 || (uintptr_t)t->k_norm % 8 || (t->rotary_dim && ((uintptr_t)t->cos % 8 || (uintptr_t)t->sin % 8)))
+        return q38_report("paged append: norms, cos and sin must be 8-byte aligned");
     if (!(t->eps >= 0.0f)) return q38_report("paged append: eps must not be negative");
     PagedAppendArgs a{};
     a.c = *c;
@@ -404,7 +407,7 @@ int q38_paged_append(const q38_paged_cache* c, const q38_paged_rows* r, const q3
 }
 
 size_t q38_paged_attention_scratch(const q38_paged_cache* c, const q38_paged_rows* r, int q_heads) {
-    if (paged_bad(c, r) || q_heads < 1 || q_heads % c->kv_heads || q_heads / c->kv_heads > 64) return 0;
+    if (paged_bad(c, r) || q_heads < 1 || q_heads % c->kv_heads || q_heads / c->kv_heads > 64 || !paged_attention_fits(*c, *r, q_heads)) return 0;
     return paged_attention_plan(*c, *r, q_heads).bytes;
 }
 
@@ -419,6 +422,7 @@ int q38_paged_attention(const q38_paged_cache* c, const q38_paged_rows* r, const
     if (q->window < 0) return q38_report("paged attention: window must not be negative");
     if (q->window && q->prefix) return q38_report("paged attention: a window and a prefix exclude each other");
     if ((uintptr_t)q->q % 16 || (uintptr_t)q->out % 16) return q38_report("paged attention: queries and outputs must be 16-byte aligned");
+    if (!paged_attention_fits(*c, *r, q->q_heads)) return q38_report("paged attention: query rows too many for one call");
     PagedAttnArgs a{};
     a.c = *c;
     a.r = *r;

@@ -19,6 +19,20 @@ constexpr float LOG2E = 1.44269504088896340736f, SLACK = 8.0f;
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
+// Sum over the lanes up to this one: within rows of 16 lanes by shifts, then each row's last lane added to the rows after it. (By
+// ds_bpermute the six steps take some 400 clocks, and a tile's lookup has three such sums one after another.)
+__device__ __forceinline__ uint32_t lanes_up_to(uint32_t x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast 15 into rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast 31 into rows 2 and 3
+    return x;
+}
+
+__device__ __forceinline__ int lane_of(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }  // lane: uniform
+
 // A workgroup's row: the same in every lane, and known to be.
 __device__ __forceinline__ PagedRow paged_row_uniform(const PagedRows& a, int row, int page_size) {
     const PagedRow r = paged_row(a, row, page_size);
@@ -47,16 +61,14 @@ __device__ __forceinline__ v8bf16 paged_widen(uint32_t w0, uint32_t w1, float sc
     return __builtin_bit_cast(v8bf16, r);
 }
 
-typedef __bf16 v4bf16 __attribute__((ext_vector_type(4)));
+// A page's scale; of one that no token wrote it may be any byte, and stays finite, so that zeros times it are zeros.
+__device__ __forceinline__ float paged_scale(int byte) { return __uint_as_float((uint32_t)min(byte, 254) << 23); }
 
-__device__ __forceinline__ v4bf16 paged_widen2(uint32_t w, float scale) {
-    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-    const u2 r = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false)),
-                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true))};
-    return __builtin_bit_cast(v4bf16, r);
+// Of a word with four positions' bytes those from `from` on and below `to`.
+__device__ __forceinline__ uint32_t paged_bytes(int from, int to) {
+    auto below = [](int n) { return n >= 4 ? 0xffffffffu : n <= 0 ? 0u : (1u << 8 * n) - 1; };
+    return below(to) & ~below(from);
 }
-
-__device__ __forceinline__ float paged_scale(int byte) { return __uint_as_float((uint32_t)byte << 23); }
 
 // Scores to powers of two: capped and biased as the call asks.
 template <int N>
@@ -65,14 +77,13 @@ __device__ __forceinline__ void paged_scores(const PagedAttnArgs& a, float (&s)[
         const float in = a.scale * 2.0f * LOG2E / a.cap, out = a.cap * LOG2E;  // tanh x = 1 - 2 / (e^2x + 1)
 #pragma unroll
         for (int e = 0; e < N; ++e) s[e] = out - 2.0f * out * __builtin_amdgcn_rcpf(exp2_(s[e] * in) + 1.0f);
+        if (a.slopes)
+#pragma unroll
+            for (int e = 0; e < N; ++e) s[e] += slope2 * (float)(j0 + e - at);
     } else {
-        const float f = a.scale * LOG2E;
+        const float f = a.scale * LOG2E, bias = slope2 * (float)(j0 - at);  // 0 without slopes
 #pragma unroll
-        for (int e = 0; e < N; ++e) s[e] *= f;
-    }
-    if (a.slopes) {
-#pragma unroll
-        for (int e = 0; e < N; ++e) s[e] += slope2 * (float)(j0 + e - at);
+        for (int e = 0; e < N; ++e) s[e] = __builtin_fmaf(s[e], f, __builtin_fmaf(slope2, (float)e, bias));
     }
 }
 
@@ -86,12 +97,15 @@ __device__ __forceinline__ void paged_scores(const PagedAttnArgs& a, float (&s)[
 // as they stand, without moving between lanes); values are A of the second product, sixteen positions of a dim being one 16-byte load.
 // Nothing goes through LDS until a workgroup's four waves, which take tiles in turn, put their sums together.
 //
-// Bound: the cache's bytes from memory. With one tile of query rows two waves per SIMD keep 64 KB of loads in flight per
-// SIMD's pair; with more, the sums and the queries take a wave's whole register file, and one wave per SIMD.
+// Bound: the cache's bytes from memory. With one tile of query rows two waves share a SIMD, with a tile's loads in flight each (16
+// or 32 KB); with more, the sums and the queries take the whole register file, and one wave is left. 64 rows of 8,192 positions, 4 KV
+// heads of 256 and six query heads to each: 187 us, 5.0 TB/s; 16 rows of 4 tokens after 32,768: 210 us, 4.5 TB/s; one row of 262,144
+// positions, 8 heads of 128: 116 us, 4.6 TB/s. Blocks of 16 positions per lane group (PT) where the registers hold them,
+// 8 for heads of 256: with 16 those spilled (decode 197 us, verify 237).
 //
-// The work is cut on the device, where the lengths are: units of 256 positions (a tile for each wave) of every row and KV head, as many per workgroup
-// as give PAGED_PER_CU workgroups per CU, rows in order. A (row, KV head) that one workgroup has all of is written out by it; the others'
-// sums go to scratch slots, which paged_join_kernel puts together.
+// The work is cut on the device, where the lengths are: units of 256 positions (a tile for each wave) of every row and KV head, as
+// many per workgroup as give PAGED_PER_CU workgroups per CU, rows in order. A (row, KV head) that one workgroup has all of is written
+// out by it; the others' sums go to scratch slots, which paged_join_kernel puts together.
 namespace {
 
 constexpr int PAGED_PER_CU = 4;  // workgroups that the work is cut into, per CU
@@ -121,16 +135,12 @@ __device__ __forceinline__ bool paged_item(const PagedAttnArgs& a, int id, int G
     for (int base = 0; base < a.r.rows; base += 64) {
         const int row = base + lane;
         const int units = base == 0 ? units0 : row < a.r.rows ? paged_units(a, row, G) : 0, n = (units + per - 1) / per, m = n > 1 ? n : 0;
-        int ends = n, slot_ends = m;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int x = __shfl_up(ends, o), y = __shfl_up(slot_ends, o);
-            if (lane >= o) ends += x, slot_ends += y;
-        }
+        const int ends = lanes_up_to(n), slot_ends = lanes_up_to(m);
         const unsigned long long past = __ballot(before + ends * Hkv > id);
         if (past) {
             const int l = __ffsll(past) - 1;
-            const int chunks = __shfl(n, l), first = before + (__shfl(ends, l) - chunks) * Hkv, slot0 = slots + (__shfl(slot_ends, l) - (chunks > 1 ? chunks : 0)) * Hkv;
+            const int chunks = lane_of(n, l), first = before + (lane_of(ends, l) - chunks) * Hkv,
+                      slot0 = slots + (lane_of(slot_ends, l) - (chunks > 1 ? chunks : 0)) * Hkv;
             it.row = base + l;
             it.chunks = chunks;
             it.kvh = (id - first) / chunks;
@@ -138,8 +148,8 @@ __device__ __forceinline__ bool paged_item(const PagedAttnArgs& a, int id, int G
             it.slot = chunks > 1 ? slot0 + id - first : -1;
             return true;
         }
-        before += __shfl(ends, 63) * Hkv;
-        slots += __shfl(slot_ends, 63) * Hkv;
+        before += lane_of(ends, 63) * Hkv;
+        slots += lane_of(slot_ends, 63) * Hkv;
     }
     return false;
 }
@@ -296,12 +306,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT > 1 ? 1 
                     sum[nt] += s[nt][e];
                 }
             }
-            if (base + TILE > total || __any(idv < 0)) {  // bytes that no token wrote may be anything
-                const int live = idv < 0 ? 0 : total - mine;
+            // What no token of the row sees may be anything: bytes behind its end, a freed page's before its window. Weight zero times
+            // NaN is none.
+            if (base + TILE > total || base < lo_all || __any(idv < 0)) {
+                const int first = lo_all - mine, live = idv < 0 ? 0 : total - mine;
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
 #pragma unroll
-                    for (int x = 0; x < PT / 4; ++x) vr[d][x] &= live >= 4 * x + 4 ? 0xffffffffu : live <= 4 * x ? 0u : (1u << 8 * (live - 4 * x)) - 1;
+                    for (int x = 0; x < PT / 4; ++x) vr[d][x] &= paged_bytes(first - 4 * x, live - 4 * x);
             }
             v8bf16 pf[NT][PT / 8];
 #pragma unroll
@@ -411,22 +423,28 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) 
 
 // ---- Many query rows (prefill chunks): tiles of 256 query rows (tokens x the KV head's query heads) per workgroup.
 //
-// A wave has 64 query rows as two 32-column B operands; keys are A, a sub-block of 32 positions at a time, its rows permuted so
-// that a lane's scores are the eight consecutive positions that it feeds to each step of weights x V, where values are A (a
-// lane then holds four consecutive dims of one query row). Each tile of positions is read from its pages once per workgroup,
-// widened to bf16 by its threads and put into one of three LDS buffers, from which the four waves read it: widening in the
-// waves' own registers would take as long as their MFMAs. 64 rows per wave, because with 32 the waves' LDS reads take as long as
-// their MFMAs (16 KB per 16 MFMAs). Sub-block i + 1's scores go before sub-block i's weights x V, beside whose MFMAs i + 1's weights
-// are formed; the next tile but one is widened beside the scores' MFMAs.
+// A wave has 32 query rows as a B operand's columns; keys are A, 32 positions at a time, their rows permuted so that a lane's
+// scores are the eight consecutive positions that it feeds to each step of weights x V, where values are A (a lane then holds
+// four consecutive dims of one query row). Each tile of 32 positions is read from its pages once per workgroup, widened to bf16 by
+// its threads and put into one of three LDS buffers, from which its eight waves read it: widening in the waves' own registers
+// would take as long as their MFMAs. Two waves share a SIMD, one half a tile behind the other, so that one's exponentials
+// run beside the other's MFMAs.
 //
-// While tiles are few, the sub-blocks of all of them, one after another, are dealt out to the CUs in equal parts: a workgroup
-// ends one tile, takes some whole and begins another. What it has of a tile that others share goes to scratch in float32
-// (256 KB for heads of 256, a dozen sub-blocks' time), and paged_join_tiles_kernel puts it together.
+// Bound: the matrix cores and the exponentials together. A tile of heads of 256 takes 4,100 to 4,500 clocks, of which its MFMAs
+// are 2,048 (2,048 tokens after 14,336, 24 and 4 heads of 256: 0.75 to 0.85 ms, 0.9 to 1.0 PFLOP/s); of heads of 128 some 2,850, of
+// which 1,024; of heads of 64, whose registers let two workgroups share a CU, 1,300 of 512. Four waves of 64 rows read LDS half
+// as often, but have no second wave to fill a SIMD's pauses: 0.83 ms.
+//
+// While tiles are few, the sub-blocks of 32 positions of all of them, one after another, are dealt out to the CUs in equal
+// parts: a workgroup ends one tile, takes some whole and begins another. What it has of a tile that others share goes to scratch
+// in float32 (256 KB for heads of 256, a dozen sub-blocks' time), and paged_join_tiles_kernel puts it together.
 namespace {
 
 constexpr int PT_TILE = 256;
-constexpr int PT_FEW = 3;    // tiles per CU: with as many they go whole, a workgroup each
-constexpr int PT_LEAST = 16;  // sub-blocks of a part
+constexpr int PT_FEW = 3;  // tiles per CU: with as many they go whole, a workgroup each
+// Sub-blocks of a part. Beginning a tile costs some 15,000 clocks (its work found, its first pages and queries read), as much as
+// five sub-blocks of heads of 128: 777 tokens after none in parts of 12 took 78 us, of 8 (more of them) 59, whole 46.
+constexpr int PT_LEAST = 16;
 constexpr int PT_PER_CU(int head_dim) { return head_dim > 64 ? 1 : 2; }  // workgroups that a CU holds
 __device__ __forceinline__ v8bf16 paged_frag(uint32_t at) {
     return *(const __attribute__((address_space(3))) v8bf16*)(uintptr_t)at;
@@ -446,14 +464,25 @@ __device__ __forceinline__ int paged_row_tiles(const PagedAttnArgs& a, const Pag
     return r.n <= 0 || (a.plan.items && r.n * G <= a.plan.few) ? 0 : (r.n * G + PT_TILE - 1) / PT_TILE;
 }
 
+// a / b of 0 <= a < 2^52, b > 0: rounding the reciprocal and the product leaves the quotient one off at most.
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+    long long q = (long long)((double)a * (1.0 / (double)b));
+    const long long left = a - q * b;
+    return left < 0 ? q - 1 : left >= b ? q + 1 : q;
+}
+
 // The call's work: `total` units, sub-blocks of its tiles in order (row, tile, KV head) or, `whole`, tiles; in equal `parts`, one
 // per workgroup.
 struct PagedWork {
     long long total;
     int jobs, parts;
     bool whole;
-    __device__ __forceinline__ long long start(int w) const { return total * w / parts; }
-    __device__ __forceinline__ int part(long long u) const { return (int)(((u + 1) * parts - 1) / total); }  // that unit u is in
+    long long each, longer;  // units of a part; the first `longer` have one more
+    __device__ __forceinline__ long long start(int w) const { return each * w + min((long long)w, longer); }
+    __device__ __forceinline__ int part(long long u) const {  // that unit u is in
+        const long long l = longer * (each + 1);
+        return u < l ? (int)quotient(u, each + 1) : (int)(longer + quotient(u - l, each));
+    }
 };
 
 // The tile that unit u of the call's work is in, and its first unit.
@@ -478,13 +507,7 @@ __device__ __forceinline__ PagedJob paged_tiles_list(const PagedAttnArgs& a, int
         const int at = min(base + lane, a.r.rows - 1);
         PagedRow r = paged_row(a.r, at, a.c.page_size);
         const int prefix = a.prefix ? a.prefix[at] : 0, n = base + lane < a.r.rows ? paged_row_tiles(a, r, G) : 0;
-        int ends = n;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int x = __shfl_up(ends, o);
-            if (lane >= o) ends += x;
-        }
-        const int count = uniform(__shfl(ends, 63));
+        const int ends = lanes_up_to(n), count = lane_of(ends, 63);
         for (int k0 = 0; k0 < count; k0 += 64) {
             const int k = k0 + lane;
             int l = 0;  // the first lane whose rows' tiles end past k
@@ -501,25 +524,20 @@ __device__ __forceinline__ PagedJob paged_tiles_list(const PagedAttnArgs& a, int
             const PagedSpan s = paged_span(a, mine, __shfl(prefix, l), max(tile, 0), G);
             const int units = k >= count ? 0 : whole ? 1 : max(1, s.hi - s.lo);
             longest = max(longest, units);
-            long long sum = units;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const long long x = __shfl_up(sum, o);
-                if (lane >= o) sum += x;
-            }
-            const unsigned long long past = find ? __ballot(before + sum * Hkv > u) : 0;
+            const uint32_t sum = lanes_up_to(units);  // of 64 tiles of up to 2^25 sub-blocks and a token's
+            const unsigned long long past = find ? __ballot(before + (long long)sum * Hkv > u) : 0;
             if (past) {
                 const int f = __ffsll(past) - 1;
                 PagedJob job;
-                job.row = base + uniform(__shfl(l, f));
-                job.tile = uniform(__shfl(tile, f));
-                job.units = uniform(__shfl(units, f));
-                const long long first = before + uniform(__shfl(sum - units, f)) * Hkv;
-                job.kvh = (int)((u - first) / job.units);
+                job.row = base + lane_of(l, f);
+                job.tile = lane_of(tile, f);
+                job.units = lane_of(units, f);
+                const long long first = before + (long long)(uint32_t)lane_of(sum - units, f) * Hkv;
+                job.kvh = (int)quotient(u - first, job.units);
                 job.start = first + (long long)job.kvh * job.units;
                 return job;
             }
-            before += uniform(__shfl(sum, 63)) * (find ? Hkv : 1);
+            before += (long long)(uint32_t)lane_of(sum, 63) * (find ? Hkv : 1);
         }
         tiles += count;
     }
@@ -532,8 +550,10 @@ __device__ __forceinline__ PagedWork paged_work(const PagedAttnArgs& a, int G) {
     const PagedJob all = paged_tiles_list(a, G, false, 0, false);
     const int jobs = all.tile * a.c.kv_heads;
     const long long total = all.start * a.c.kv_heads;
-    if (!a.plan.parts || jobs >= PT_FEW * a.plan.cus || all.units <= 2 * PT_LEAST) return {jobs, jobs, jobs, true};
-    return {total, jobs, (int)max(1LL, min((long long)a.plan.parts, total / PT_LEAST)), false};
+    if (!a.plan.parts || jobs >= PT_FEW * a.plan.cus || all.units <= 2 * PT_LEAST) return {jobs, jobs, jobs, true, 1, 0};
+    const int parts = (int)max(1LL, min((long long)a.plan.parts, total / PT_LEAST));
+    const long long each = quotient(total, parts);
+    return {total, jobs, parts, false, each, total - each * parts};
 }
 
 // A cut tile in the scratch's table, at the workgroup that begins it: which workgroups' sums make it.
@@ -566,6 +586,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2 * PT_PER_
     if (job.row < 0) return;
     const PagedRow r = paged_row_uniform(a.r, job.row, ps);
     const int R = r.n * G, total = r.p0 + r.n, prefix = a.prefix ? uniform(a.prefix[job.row]) : 0;
+    const int lo_all = a.window ? max(0, r.p0 + 1 - a.window) : 0;
     const int* table = a.r.pages + (size_t)job.row * a.r.max_pages;
     // This part's tiles of 32 positions of those that any of the workgroup's query rows sees.
     const PagedSpan span = paged_span(a, r, prefix, job.tile, G);
@@ -605,10 +626,11 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2 * PT_PER_
     const int c0 = (int)threadIdx.x & (PIECES - 1), vg0 = uniform(c0 / HD);
     uint4 rk, rv;
     int id, found, ks, vs;  // this tile's page; the next one's as read; scale bytes
-    // A tile's page number is read a tile before its keys and values, so that no load waits for another.
-    auto look = [&](int T) __attribute__((always_inline)) { found = table[min((T * 32 + vg0 * 16) >> shift, a.r.max_pages - 1)]; };
+    // Tiles go from the part's last to its first: the nearest positions first, whose scores are the largest where distance takes from
+    // them. A tile's page number is read a tile before its keys and values, so that no load waits for another.
+    auto look = [&](int T) __attribute__((always_inline)) { found = table[min((max(T, T0) * 32 + vg0 * 16) >> shift, a.r.max_pages - 1)]; };
     auto load = [&](int T) __attribute__((always_inline)) {
-        const int p = T * 32 + vg0 * 16;
+        const int p = max(T, T0) * 32 + vg0 * 16;
         id = uniform(found);
         id = ((id < a.c.pages) & (p >> shift < a.r.max_pages)) ? id : -1;
         const size_t hd = (size_t)max(id, 0) * Hkv + job.kvh, at = (hd * ps + (p & (ps - 1))) * HD + c0 % HD * 16;
@@ -622,26 +644,26 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2 * PT_PER_
             rk = *(const uint4*)((keys ? a.c.k : a.c.v) + at);
         }
     };
-    // Step x of widening the loaded tile T into its buffer. Keys: row (position), its 16-byte chunks spread over the banks;
+    // Step x of widening the loaded tile T into buffer b. Keys: row (position), its 16-byte chunks spread over the banks;
     // values: per dim 32 positions, likewise.
     const uint32_t lds0 = (uint32_t)(uintptr_t)LDS_PTR(&ring[0]);
     const int kp0 = c0 / (HD / 16), kc0 = c0 % (HD / 16) * 2, vd0 = c0 % HD;
     const uint32_t put_k = kp0 * HD * 2 + ((kc0 ^ (HD > 64 ? kp0 & 15 : (kp0 >> 1) & 7)) << 4);
     const uint32_t put_v = HALF + vd0 * 64 + ((vg0 * 2 ^ ((vd0 >> 1) & 3) ^ ((vd0 >> 3) & 1)) << 4);
-    auto widen = [&](int T, int x) __attribute__((always_inline)) {
-        const uint32_t buf = lds0 + T % 3 * BUF;
+    auto widen = [&](int T, int b, int x) __attribute__((always_inline)) {
+        const uint32_t buf = lds0 + b * BUF;
         const int u = x & 1;
         const bool key = BOTH ? x < 2 : keys;
         if (x == 0) {
-            // Bytes that no token wrote may be anything, and so may those of a page that is not there.
-            if ((T * 32 + 32 > total) | (id < 0)) {
-                const int left = id < 0 ? 0 : total - (T * 32 + vg0 * 16);
+            // What no token of the row sees may be anything: weight zero times NaN is none.
+            if ((T * 32 + 32 > total) | (T * 32 < lo_all) | (id < 0)) {
+                const int at = T * 32 + vg0 * 16, first = lo_all - at, left = id < 0 ? 0 : total - at;
                 uint32_t* w4 = (uint32_t*)(BOTH ? &rv : &rk);
                 if (vals)
 #pragma unroll
-                    for (int y = 0; y < 4; ++y) w4[y] &= left >= 4 * y + 4 ? 0xffffffffu : left <= 4 * y ? 0u : (1u << 8 * (left - 4 * y)) - 1;
+                    for (int y = 0; y < 4; ++y) w4[y] &= paged_bytes(first - 4 * y, left - 4 * y);
             }
-            if (vd0 == 0) lost[T % 3][vg0] = id < 0;
+            if (vd0 == 0) lost[b][vg0] = id < 0;
         }
         const uint4 w4 = !BOTH || key ? rk : rv;
         const uint32_t at = key ? put_k ^ (u << 4) : put_v ^ (u << 4);
@@ -672,10 +694,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2 * PT_PER_
         asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(x), "v"(y), "v"(z));
         return m;
     };
-    // Scores of tile T, with the loaded tile T + 1 widened beside their MFMAs and the one after it asked for; then its weights.
-    auto scores = [&](int T) __attribute__((always_inline)) {
-        const uint32_t ka = lds0 + T % 3 * BUF + kl;
-        const int gone0 = lost[T % 3][0], gone1 = lost[T % 3][1];
+    // Scores of tile T in buffer b, with the loaded tile T - 1 widened beside their MFMAs and the one after it asked for; then its weights.
+    auto scores = [&](int T, int b, int next) __attribute__((always_inline)) {
+        const uint32_t ka = lds0 + b * BUF + kl;
+        const int gone0 = lost[b][0], gone1 = lost[b][1];
         v8bf16 kf[DEEP], qx[DEEP];
         v16f c[CHAINS], zero;
 #pragma unroll
@@ -692,11 +714,11 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2 * PT_PER_
             c[m % CHAINS] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[m % DEEP], q, m < CHAINS ? zero : c[m % CHAINS], 0, 0, 0);
             if (m + DEEP < QS) qx[m % DEEP] = q_wait[(m + DEEP) * 512 + threadIdx.x];
             if (m + DEEP < KM) kf[m % DEEP] = paged_frag(ka ^ ((m + DEEP) << 5));
-            if (m >= KM - STEPS) widen(T + 1, m - (KM - STEPS));
+            if (m >= KM - STEPS) widen(T - 1, next, m - (KM - STEPS));
         }
         __builtin_amdgcn_sched_barrier(0);
-        load(min(T + 2, T1 - 1));
-        look(min(T + 3, T1 - 1));
+        load(T - 2);
+        look(T - 3);
         s = CHAINS > 1 ? c[0] + c[CHAINS - 1] : c[0];
         const int p0 = T * 32, lost0 = uniform(gone0), lost1 = uniform(gone1);
         if (bent)
@@ -736,9 +758,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2 * PT_PER_
             pw[e >> 3][(e >> 1) & 3] = pk_bf16(p, q);
         }
     };
-    // Weights x V of tile T.
-    auto values = [&](int T) __attribute__((always_inline)) {
-        const uint32_t va = lds0 + T % 3 * BUF + vl;
+    // Weights x V of the tile in buffer b.
+    auto values = [&](int b) __attribute__((always_inline)) {
+        const uint32_t va = lds0 + b * BUF + vl;
         auto frag = [&](int x) __attribute__((always_inline)) { return paged_frag((va ^ (x / VD << 5)) + x % VD * 2048); };
         v8bf16 vf[DEEP];
 #pragma unroll
@@ -761,22 +783,24 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2 * PT_PER_
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
         if (T0 >= T1) break;
-        look(T0);
-        load(T0);
-        look(min(T0 + 1, T1 - 1));
+        look(T1 - 1);
+        load(T1 - 1);
+        look(T1 - 2);
 #pragma unroll
-        for (int x = 0; x < STEPS; ++x) widen(T0, x);
-        load(min(T0 + 1, T1 - 1));
-        look(min(T0 + 2, T1 - 1));
-        // Tile T is in buffer T % 3, widened there before its beginning, which the first four waves meet before their scores of it, the
+        for (int x = 0; x < STEPS; ++x) widen(T1 - 1, 0, x);
+        load(T1 - 2);
+        look(T1 - 3);
+        // The buffers go round. A tile is in its own, widened there before its beginning, which the first four waves meet before their scores of it, the
         // other four, which share the SIMDs with them, before their weights x V of the tile before: so one of a SIMD's two waves
         // forms weights while the other feeds the matrix cores. A tile goes into the buffer of the one three before, whose
         // last weights x V lie before the meeting before.
-        for (int T = T0; T < T1; ++T) {
-            if (wv < 4 || T == T0) meet();
-            scores(T);
-            if (wv >= 4 && T + 1 < T1) meet();
-            values(T);
+        for (int T = T1 - 1, b = 0; T >= T0; --T) {
+            const int next = b == 2 ? 0 : b + 1;
+            if (wv < 4 || T == T1 - 1) meet();
+            scores(T, b, next);
+            if (wv >= 4 && T > T0) meet();
+            values(b);
+            b = next;
         }
         most = fmaxf(most, __shfl_xor(most, 32)) * mul;
         if (pass || !__syncthreads_or(most > top + LEAP)) break;
@@ -870,6 +894,11 @@ PagedPlan paged_attention_plan(const PagedCache& c, const PagedRows& r, int q_he
         }
     }
     return p;
+}
+
+// A grid's threads are counted in 32 bits.
+bool paged_attention_fits(const PagedCache& c, const PagedRows& r, int q_heads) {
+    return (long long)r.rows * c.kv_heads * (((long long)r.max_tokens * (q_heads / c.kv_heads) + PT_TILE - 1) / PT_TILE) < 1 << 23;
 }
 
 hipError_t q38_paged_attention(const PagedAttnArgs& a, hipStream_t stream) {

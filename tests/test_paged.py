@@ -123,3 +123,32 @@ def test_an_engine_sizes_its_paged_caches_and_refuses_others():
         kw = {"max_seq_len": 128, "kv_cache_format": "fp8", "kv_pages": 8, "kv_page_size": 64, **changes}
         with pytest.raises(RuntimeError, match=message):
             ext.Handle(cfg, 4, 4, kw.pop("max_seq_len"), True, **kw)
+
+
+def test_calls_too_large_for_a_grid_are_refused():
+    lib, ref = ext.library(), ctypes.byref
+    c, r, t, q = args(c__kv_heads=4, q__q_heads=4, r__rows=1 << 16, r__tokens=1 << 17, r__max_tokens=2)
+    assert "rows * kv_heads too large" in error(lib.q38_paged_append(ref(c), ref(r), ref(t), None))
+    assert "rows * kv_heads too large" in error(lib.q38_paged_attention(ref(c), ref(r), ref(q), P, 1 << 60, None))
+    assert lib.q38_paged_attention_scratch(ref(c), ref(r), 4) == 0
+    c, r, t, q = args(c__kv_heads=16, q__q_heads=1024, r__rows=1, r__tokens=1 << 22, r__max_tokens=1 << 22)
+    assert "query rows too many" in error(lib.q38_paged_attention(ref(c), ref(r), ref(q), P, 1 << 60, None))
+    assert lib.q38_paged_attention_scratch(ref(c), ref(r), 1024) == 0
+
+
+@pytest.mark.parametrize("changes, message", [
+    ({"t__cos": P + 4}, "aligned"), ({"t__sin": P + 2}, "aligned"), ({"t__q_norm": P + 4}, "aligned"), ({"t__k_norm": P + 2}, "aligned")])
+def test_append_refuses_misaligned_vectors(changes, message):
+    c, r, t, _ = args(**changes)
+    assert message in error(ext.library().q38_paged_append(ctypes.byref(c), ctypes.byref(r), ctypes.byref(t), None))
+
+
+def test_a_scratch_that_is_too_small_or_misaligned_is_refused():
+    lib, ref = ext.library(), ctypes.byref
+    for changes in ({}, {"r__max_tokens": 10}):
+        c, r, _, q = args(**changes)
+        need = lib.q38_paged_attention_scratch(ref(c), ref(r), 4)
+        assert need > 0
+        assert "scratch is smaller" in error(lib.q38_paged_attention(ref(c), ref(r), ref(q), P, need - 1, None))
+        assert "scratch is smaller" in error(lib.q38_paged_attention(ref(c), ref(r), ref(q), None, need, None))
+        assert "256-byte" in error(lib.q38_paged_attention(ref(c), ref(r), ref(q), P + 128, need, None))
