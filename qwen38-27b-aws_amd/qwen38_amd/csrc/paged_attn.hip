@@ -223,12 +223,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT > 1 ? 1 
     auto find = [&](int t, int group) { return paged_find(a.r, table, (t * TILE + group * PT) >> shift, a.c.pages); };
     uint4 kr[NB][KB];
     words vr[DB];
-    float ks, vs;
+    int ks, vs;  // scale bytes: made scales where they are used, as doing it here would wait for them
     auto load_keys = [&](int t, int id) __attribute__((always_inline)) {
         const size_t head = (size_t)max(id, 0) * Hkv + it.kvh;
         const int slot = (t * TILE + (col >> 2) * PT + (col & 3)) & (ps - 1);
         const uint8_t* p = a.c.k + (head * ps + slot) * HD + g * 16;
-        ks = paged_scale(a.c.k_scale[head]);
+        ks = a.c.k_scale[head];
 #pragma unroll
         for (int j = 0; j < KB; ++j)
 #pragma unroll
@@ -238,7 +238,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT > 1 ? 1 
         const size_t head = (size_t)max(id, 0) * Hkv + it.kvh;
         const int slot = (t * TILE + g * PT) & (ps - 1);
         const uint8_t* p = a.c.v + head * ps * HD + ((size_t)(slot >> 4) * HD + col) * 16 + (slot & 15);
-        vs = paged_scale(a.c.v_scale[head]);
+        vs = a.c.v_scale[head];
 #pragma unroll
         for (int d = 0; d < DB; ++d) vr[d] = *(const words*)(p + d * 256);
     };
@@ -254,7 +254,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT > 1 ? 1 
             float s[NT][PT];
             {
                 v4f c[NT][NB];
-                const float scale = ks;
+                const float scale = paged_scale(ks);
 #pragma unroll
                 for (int j = 0; j < KB; ++j) {
                     __builtin_amdgcn_sched_barrier(0);
@@ -325,7 +325,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT > 1 ? 1 
                                   pk_bf16(s[nt][8 * u + 4], s[nt][8 * u + 5]), pk_bf16(s[nt][8 * u + 6], s[nt][8 * u + 7])};
                     pf[nt][u] = __builtin_bit_cast(v8bf16, w);
                 }
-            const float scale = vs;
+            const float scale = paged_scale(vs);
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
                 if (d % 4 == 0) __builtin_amdgcn_sched_barrier(0);
