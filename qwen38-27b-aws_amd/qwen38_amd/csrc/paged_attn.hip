@@ -570,7 +570,6 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2 * PT_PER_
     constexpr bool BOTH = HD == 256;
     constexpr int STEPS = BOTH ? 4 : 2;  // half pieces to widen
     constexpr int DEEP = HD > 128 ? 2 : 4;  // operands read ahead from LDS
-    constexpr int CHAINS = HD > 128 ? 1 : 2;  // sums that a score is made of
     __shared__ __attribute__((aligned(1024))) uint8_t ring[3 * BUF];
     __shared__ int lost[3][2];
     __shared__ float slopes[PT_TILE];
@@ -626,6 +625,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2 * PT_PER_
     const int c0 = (int)threadIdx.x & (PIECES - 1), vg0 = uniform(c0 / HD);
     uint4 rk, rv;
     int id, found, ks, vs;  // this tile's page; the next one's as read; scale bytes
+    // Zero, but not for the compiler: it would take the scale bytes for uniform and move them to scalar registers as soon as they
+    // are asked for, which waits for them in every tile.
+    uint32_t zero;
+    asm("v_mov_b32 %0, 0" : "=v"(zero));
     // Tiles go from the part's last to its first: the nearest positions first, whose scores are the largest where distance takes from
     // them. A tile's page number is read a tile before its keys and values, so that no load waits for another.
     auto look = [&](int T) __attribute__((always_inline)) { found = table[min((max(T, T0) * 32 + vg0 * 16) >> shift, a.r.max_pages - 1)]; };
@@ -635,12 +638,12 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2 * PT_PER_
         id = ((id < a.c.pages) & (p >> shift < a.r.max_pages)) ? id : -1;
         const size_t hd = (size_t)max(id, 0) * Hkv + job.kvh, at = (hd * ps + (p & (ps - 1))) * HD + c0 % HD * 16;
         if constexpr (BOTH) {
-            ks = a.c.k_scale[hd];
-            vs = a.c.v_scale[hd];
+            ks = (a.c.k_scale + hd)[zero];
+            vs = (a.c.v_scale + hd)[zero];
             rk = *(const uint4*)(a.c.k + at);
             rv = *(const uint4*)(a.c.v + at);
         } else {
-            ks = (keys ? a.c.k_scale : a.c.v_scale)[hd];
+            ks = ((keys ? a.c.k_scale : a.c.v_scale) + hd)[zero];
             rk = *(const uint4*)((keys ? a.c.k : a.c.v) + at);
         }
     };
@@ -699,9 +702,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2 * PT_PER_
         const uint32_t ka = lds0 + b * BUF + kl;
         const int gone0 = lost[b][0], gone1 = lost[b][1];
         v8bf16 kf[DEEP], qx[DEEP];
-        v16f c[CHAINS], zero;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) zero[e] = 0.0f;
+        for (int e = 0; e < 16; ++e) s[e] = 0.0f;
 #pragma unroll
         for (int m = 0; m < DEEP; ++m) {
             kf[m] = paged_frag(ka ^ (m << 5));
@@ -711,7 +713,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2 * PT_PER_
         for (int m = 0; m < KM; ++m) {
             __builtin_amdgcn_sched_barrier(0);
             const v8bf16 q = m < QS ? qx[m % DEEP] : qf[m];
-            c[m % CHAINS] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[m % DEEP], q, m < CHAINS ? zero : c[m % CHAINS], 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[m % DEEP], q, s, 0, 0, 0);
             if (m + DEEP < QS) qx[m % DEEP] = q_wait[(m + DEEP) * 512 + threadIdx.x];
             if (m + DEEP < KM) kf[m % DEEP] = paged_frag(ka ^ ((m + DEEP) << 5));
             if (m >= KM - STEPS) widen(T - 1, next, m - (KM - STEPS));
@@ -719,7 +721,6 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2 * PT_PER_
         __builtin_amdgcn_sched_barrier(0);
         load(T - 2);
         look(T - 3);
-        s = CHAINS > 1 ? c[0] + c[CHAINS - 1] : c[0];
         const int p0 = T * 32, lost0 = uniform(gone0), lost1 = uniform(gone1);
         if (bent)
 #pragma unroll
