@@ -387,13 +387,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT > 1 ? 1 
     }
 }
 
-// The parts of one (row, KV head)'s query row put together. Grid: rows x KV heads x query rows.
-template <int E>
-__global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) {
+// The parts of one (row, KV head)'s query row put together, W waves every W-th of them each, four under way at a time. Grid: rows x
+// KV heads x query rows. Sixteen waves where parts are many (one row of 262,144 positions has 128 per KV head: 7 us against 15 with
+// four waves), four where they are few and the workgroups many (64 rows of 8,192 positions: 189 us in all against 204 with
+// sixteen).
+template <int E, int W>
+__global__ __launch_bounds__(W * 64) void paged_join_kernel(const PagedAttnArgs a) {
     constexpr int HD = E * 64;
-    __shared__ float sums[4][HD], totals[4];
+    __shared__ float sums[W][HD], totals[W];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, Hkv = a.c.kv_heads, G = a.q_heads / Hkv;
-    const int q = blockIdx.x % a.plan.few, kvh = blockIdx.x / a.plan.few % Hkv, row = blockIdx.x / a.plan.few / Hkv;
+    const int n = a.plan.joins, q = blockIdx.x % n, kvh = blockIdx.x / n % Hkv, row = blockIdx.x / n / Hkv;
     const PagedRow r = paged_row(a.r, row, a.c.page_size);
     if (q >= r.n * G || r.n * G > a.plan.few) return;
     const int2 t = ((const int2*)(a.scratch + a.plan.table))[row * Hkv + kvh];
@@ -405,20 +408,36 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a) 
     for (int c = lane; c < t.y; c += 64) top = fmaxf(top, stats[c * step]);
     top = warp_max(top);
     float o[E] = {}, l = 0.0f;
-    for (int c = wv; c < t.y; c += 4) {
-        const float2 s = *(const float2*)(stats + c * step);
-        const float f = s.x == -INFINITY ? (s.y == 0.0f ? 0.0f : 1.0f) : exp2_(s.x - top);  // no weights, or only NaN ones
-        l += s.y * f;
+    for (int c0 = wv; c0 < t.y; c0 += 4 * W) {
+        float2 s[4];
+        float v[4][E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] += part[c * step + (size_t)q * HD + e * 64 + lane] * f;
+        for (int i = 0; i < 4; ++i) {
+            const size_t c = min(c0 + i * W, t.y - 1);
+            s[i] = *(const float2*)(stats + c * step);
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[i][e] = part[c * step + (size_t)q * HD + e * 64 + lane];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (c0 + i * W >= t.y) break;
+            const float f = s[i].x == -INFINITY ? (s[i].y == 0.0f ? 0.0f : 1.0f) : exp2_(s[i].x - top);  // no weights, or only NaN ones
+            l += s[i].y * f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] += v[i][e] * f;
+        }
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) sums[wv][e * 64 + lane] = o[e];
     if (lane == 0) totals[wv] = l;
     __syncthreads();
-    const float all = (totals[0] + totals[1]) + (totals[2] + totals[3]);
     bf16_t* out = a.out + ((size_t)(r.t0 + q / G) * a.q_heads + kvh * G + q % G) * HD;
-    for (int d = threadIdx.x; d < HD; d += 256) out[d] = f2bf(((sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d])) / all);
+    for (int d = threadIdx.x; d < HD; d += W * 64) {
+        float all = 0.0f, x = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) all += totals[w], x += sums[w][d];
+        out[d] = f2bf(x / all);
+    }
 }
 
 // ---- Many query rows (prefill chunks): tiles of 256 query rows (tokens x the KV head's query heads) per workgroup.
@@ -873,6 +892,7 @@ PagedPlan paged_attention_plan(const PagedCache& c, const PagedRows& r, int q_he
     const bool any = most <= 64 || r.q_start;
     p.target = PAGED_PER_CU * q38_device_cus();
     const long long heads = (long long)r.rows * c.kv_heads, units = ((long long)r.max_pages * c.page_size + r.max_tokens + 63) / 64 / 4 + 2;
+    p.joins = (int)std::min<long long>(most, p.few);
     p.items = any ? (int)std::min<long long>(p.target + heads, heads * units) : 0;
     p.slots = units > 1 ? std::min(2 * p.target, p.items) : 0;
     p.bytes = 0;
@@ -920,12 +940,20 @@ hipError_t q38_paged_attention(const PagedAttnArgs& a, hipStream_t stream) {
             case 256: STREAMS(256); break;
             default: return hipErrorInvalidValue;
         }
-        const size_t rows = (size_t)a.r.rows * a.c.kv_heads * few;
+        const int heads = a.r.rows * a.c.kv_heads;
+#define JOIN(E)                                                                                                              \
+    do {                                                                                                                     \
+        if (heads * 32 <= a.plan.target)                                                                                     \
+            hipLaunchKernelGGL((paged_join_kernel<E, 16>), dim3(heads * a.plan.joins), dim3(1024), 0, stream, a);            \
+        else                                                                                                                 \
+            hipLaunchKernelGGL((paged_join_kernel<E, 4>), dim3(heads * a.plan.joins), dim3(256), 0, stream, a);              \
+    } while (0)
         switch (a.plan.slots ? a.c.head_dim : 0) {
-            case 64: hipLaunchKernelGGL((paged_join_kernel<1>), dim3(rows), dim3(256), 0, stream, a); break;
-            case 128: hipLaunchKernelGGL((paged_join_kernel<2>), dim3(rows), dim3(256), 0, stream, a); break;
-            case 256: hipLaunchKernelGGL((paged_join_kernel<4>), dim3(rows), dim3(256), 0, stream, a); break;
+            case 64: JOIN(1); break;
+            case 128: JOIN(2); break;
+            case 256: JOIN(4); break;
         }
+#undef JOIN
         if ((long long)a.r.max_tokens * G <= few) return hipGetLastError();
     }
 #define TILES(HD)                                                                                                             \
