@@ -98,7 +98,7 @@ __device__ __forceinline__ void paged_scores(const PagedAttnArgs& a, float (&s)[
 // Nothing goes through LDS until a workgroup's four waves, which take tiles in turn, put their sums together.
 //
 // Bound: the cache's bytes from memory. With one tile of query rows two waves share a SIMD, with a tile's loads in flight each (16
-// or 32 KB); with more, the sums and the queries take the whole register file, and one wave is left. 64 rows of 8,192 positions, 4 KV
+// or 32 KB); with more, the sums and the queries mostly take the whole register file, and one wave is left. 64 rows of 8,192 positions, 4 KV
 // heads of 256 and six query heads to each: 187 us, 5.0 TB/s; 16 rows of 4 tokens after 32,768: 210 us, 4.5 TB/s; one row of 262,144
 // positions, 8 heads of 128: 116 us, 4.6 TB/s. Blocks of 16 positions per lane group (PT) where the registers hold them,
 // 8 for heads of 256: with 16 those spilled (decode 197 us, verify 237).
@@ -156,8 +156,12 @@ __device__ __forceinline__ bool paged_item(const PagedAttnArgs& a, int id, int G
 
 }  // namespace
 
+// Waves that share a SIMD: two while the sums and queries leave room for the loads (16 rows of 32,768 positions, 4 KV heads of 64, two and
+// three tiles 59 and 66 us against 87 and 99 with one; four tiles 131 against 120, and two tiles of heads of 128 152 against 130).
+constexpr int PAGED_WAVES(int hd, int tiles) { return tiles == 1 || hd * tiles <= 192 ? 2 : 1; }
+
 template <int HD, int NT, int PT>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT > 1 ? 1 : 2, NT > 1 ? 1 : 2))) void paged_stream_kernel(const PagedAttnArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PAGED_WAVES(HD, NT), PAGED_WAVES(HD, NT)))) void paged_stream_kernel(const PagedAttnArgs a) {
     constexpr int KB = HD / 64, DB = HD / 16, LD = HD + 4, NB = PT / 4, TILE = 4 * PT;
     typedef uint32_t words __attribute__((ext_vector_type(PT / 4)));
     __shared__ __attribute__((aligned(16))) float sums[4 * 16 * LD];
@@ -887,9 +891,12 @@ PagedPlan paged_attention_plan(const PagedCache& c, const PagedRows& r, int q_he
     PagedPlan p{};
     const int G = q_heads / c.kv_heads;
     const long long most = (long long)r.max_tokens * G;
-    // All rows stream while their query rows fit four tiles; in a ragged call with longer rows those of one tile of tokens.
-    p.few = (int)(most <= 64 ? (most + 15) / 16 * 16 : (G + 15) / 16 * 16);
-    const bool any = most <= 64 || r.q_start;
+    // All rows stream while their query rows fit four tiles, three for heads of 256 (the fourth's sums do not fit the registers: 16 rows of
+    // 32,768 positions, 64 query rows, 1,627 us against 473 as a tile of 256); in a ragged call with longer rows those of one token, or of
+    // a few while these fit one tile.
+    const int limit = c.head_dim > 128 ? 48 : 64;
+    const bool any = most <= limit || (r.q_start && G <= limit);
+    p.few = !any ? 0 : (int)((most <= limit ? most : G) + 15) / 16 * 16;
     p.target = PAGED_PER_CU * q38_device_cus();
     const long long heads = (long long)r.rows * c.kv_heads, units = ((long long)r.max_pages * c.page_size + r.max_tokens + 63) / 64 / 4 + 2;
     p.joins = (int)std::min<long long>(most, p.few);
@@ -926,20 +933,21 @@ hipError_t q38_paged_attention(const PagedAttnArgs& a, hipStream_t stream) {
     const int few = a.plan.few, G = a.q_heads / a.c.kv_heads;
     if (a.plan.items) {
 #define STREAM(HD, NT) hipLaunchKernelGGL((paged_stream_kernel<HD, NT, (HD > 128 ? 8 : 16)>), dim3(a.plan.items), dim3(256), 0, stream, a)
-#define STREAMS(HD)                  \
-    switch (few / 16) {              \
-        case 1: STREAM(HD, 1); break; \
-        case 2: STREAM(HD, 2); break; \
-        case 3: STREAM(HD, 3); break; \
-        case 4: STREAM(HD, 4); break; \
-        default: return hipErrorInvalidValue; \
-    }
-        switch (a.c.head_dim) {
-            case 64: STREAMS(64); break;
-            case 128: STREAMS(128); break;
-            case 256: STREAMS(256); break;
+        switch (a.c.head_dim * 8 + few / 16) {
+            case 64 * 8 + 1: STREAM(64, 1); break;
+            case 64 * 8 + 2: STREAM(64, 2); break;
+            case 64 * 8 + 3: STREAM(64, 3); break;
+            case 64 * 8 + 4: STREAM(64, 4); break;
+            case 128 * 8 + 1: STREAM(128, 1); break;
+            case 128 * 8 + 2: STREAM(128, 2); break;
+            case 128 * 8 + 3: STREAM(128, 3); break;
+            case 128 * 8 + 4: STREAM(128, 4); break;
+            case 256 * 8 + 1: STREAM(256, 1); break;
+            case 256 * 8 + 2: STREAM(256, 2); break;
+            case 256 * 8 + 3: STREAM(256, 3); break;
             default: return hipErrorInvalidValue;
         }
+#undef STREAM
         const int heads = a.r.rows * a.c.kv_heads;
 #define JOIN(E)                                                                                                              \
     do {                                                                                                                     \

@@ -137,6 +137,16 @@ def test_every_number_of_query_row_tiles(gpu, hd, tokens, options):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("hq, hkv", [(64, 1), (98, 2), (33, 1)])
+def test_many_query_heads_to_a_key_head(gpu, hd, hq, hkv):
+    """33, 49 and 64 of them, with one and two tokens a row, alike and not."""
+    for lengths, position in (([1, 1], [700, 3]), ([2, 2], [0, 90]), ([1, 2, 0, 1], [5, 300, 9, 44])):
+        args, call, want = attend_case(hq, hkv, hd, 32, lengths, position, {})
+        check_attention(ext.paged_attention(*args, **call), want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("hd, hq, hkv", [(64, 2, 1), (256, 64, 1), (128, 5, 5)])
 def test_many_rows(gpu, hd, hq, hkv):
     """More rows than a wave has lanes, short and long ones and none among them."""
