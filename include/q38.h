@@ -294,8 +294,8 @@ typedef struct q38_paged_cache {
  * alone), or with q_start null max_tokens each. max_tokens bounds every row's tokens (of a row with more the first max_tokens
  * are taken). position int32 [rows]: the first token's position in its row; negative skips the row (nothing is appended, its
  * outputs are zero). pages int32 [rows][max_pages]: the pages of each row's positions in order. An entry outside [0, pages), like
- * a position past the table, names no page: nothing is appended there, and a query that sees it answers NaN. Rows may share
- * pages that none of them appends to. rows * kv_heads is below 2^18, rows * max_tokens at most 2^24. */
+ * a position past the table, names no page: nothing is appended there, and a query that sees it answers NaN. A row names a page
+ * once; rows may share pages that none of them appends to. rows * kv_heads is below 2^18, rows * max_tokens at most 2^24. */
 typedef struct q38_paged_rows {
     const int32_t *position, *pages, *q_start;
     int rows, max_pages, tokens, max_tokens;
@@ -339,7 +339,8 @@ typedef struct q38_paged_query {
 } q38_paged_query;
 
 /* Attention of every row's tokens, at positions position .., over its cached positions, the tokens' own (appended before)
- * among them: softmax over the positions a token sees, float32 sums. scratch holds at least q38_paged_attention_scratch bytes
+ * among them: softmax over the positions a token sees, float32 sums (formed before they are divided: cached values beyond 2^57 may
+ * overflow them). scratch holds at least q38_paged_attention_scratch bytes
  * (256-byte aligned, contents free; null if that is 0); calls that share it must not overlap. */
 int q38_paged_attention(const q38_paged_cache* cache, const q38_paged_rows* rows, const q38_paged_query* query, void* scratch,
                         size_t scratch_bytes, void* stream);

@@ -510,6 +510,8 @@ def paged_attention(cache: PagedCache, q: torch.Tensor, position: torch.Tensor, 
     a = _QueryArgs(qp, _want("out", out, bf, shape, device), heads, hd**-0.5 if scale is None else scale, cap, window,
                    None if slopes is None else _want("slopes", slopes, torch.float32, (heads,), device),
                    None if prefix is None else _want("prefix", prefix, torch.int32, (r.rows,), device))
+    if not 0 <= window < 2**31:
+        raise ValueError(f"window must be 0 (none) to 2**31 - 1, got {window}")
     ref, lib = ctypes.byref, library()
     if scratch is None:
         size = lib.q38_paged_attention_scratch(ref(c), ref(r), heads)

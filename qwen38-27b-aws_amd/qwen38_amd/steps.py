@@ -273,8 +273,9 @@ class Engine:
         """Row ``row``'s pages in order of its positions (at most max_seq_len / kv_page_size; the places after them hold none). Rows may
         share pages that none of them appends to: those of a common prefix."""
         table = self.page_table
-        if not 0 <= row < table.shape[0] or len(pages) > table.shape[1] or any(not 0 <= p < self.kv_pages for p in pages):
-            raise ValueError(f"row {row} of {table.shape[0]} takes up to {table.shape[1]} pages out of {self.kv_pages}")
+        known = all(0 <= p < self.kv_pages for p in pages) and len(set(pages)) == len(pages)
+        if not 0 <= row < table.shape[0] or len(pages) > table.shape[1] or not known:
+            raise ValueError(f"row {row} of {table.shape[0]} takes up to {table.shape[1]} pages out of {self.kv_pages}, each once")
         table[row] = torch.tensor([*pages, *[-1] * (table.shape[1] - len(pages))], dtype=torch.int32)
 
     def kv_cache(self, layer: int) -> tuple[torch.Tensor, torch.Tensor]:

@@ -312,6 +312,8 @@ def test_what_is_refused_on_a_device(gpu):
         lambda: ext.paged_append(cache, kv, kv, position, pages, cos=torch.zeros(4, 64, dtype=BF16).cuda()),
         lambda: ext.paged_append(cache, kv, kv, position, pages, q_norm=torch.zeros(64, dtype=BF16).cuda()),
         lambda: ext.paged_append(cache, kv.transpose(1, 2), kv, position, pages),
+        lambda: ext.paged_attention(cache, q, position, pages, window=2**32 + 5),
+        lambda: ext.paged_attention(cache, q, position, pages, window=-1),
     ):
         with pytest.raises(ValueError):
             call()

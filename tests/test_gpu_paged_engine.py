@@ -228,7 +228,8 @@ def test_what_an_engine_refuses(gpu, weights):
     cfg, values = weights
     e = paged(cfg, values)
     for call in (lambda: e.get_kv(0), lambda: e.set_kv_scales(0, torch.ones(1), torch.ones(1)), lambda: e.set_pages(B, [0]),
-                 lambda: e.set_pages(0, [B * EACH + 2]), lambda: e.set_pages(0, [-1]), lambda: e.set_pages(0, [0] * (EACH + 1))):
+                 lambda: e.set_pages(0, [B * EACH + 2]), lambda: e.set_pages(0, [-1]), lambda: e.set_pages(0, list(range(EACH + 1))),
+                 lambda: e.set_pages(0, [5, 5])):
         with pytest.raises(ValueError):
             call()
     slab = Engine(cfg, B, K, S, kv_cache_format="fp8")
