@@ -892,11 +892,13 @@ PagedPlan paged_attention_plan(const PagedCache& c, const PagedRows& r, int q_he
     const int G = q_heads / c.kv_heads;
     const long long most = (long long)r.max_tokens * G;
     // All rows stream while their query rows fit four tiles, three for heads of 256 (the fourth's sums do not fit the registers: 16 rows of
-    // 32,768 positions, 64 query rows, 1,627 us against 473 as a tile of 256); in a ragged call with longer rows those of one token, or of
-    // a few while these fit one tile.
+    // 32,768 positions, 64 query rows, 1,627 us against 473 as a tile of 256). In a ragged call with longer rows those of the other
+    // rows' usual number of tokens, if that many fit, or else of one token: a single token pays for the tiles that it does not
+    // fill (heads of 256, two tiles for one 240 us against 191), a verify row that goes as a tile of 256 takes twice as long.
     const int limit = c.head_dim > 128 ? 48 : 64;
     const bool any = most <= limit || (r.q_start && G <= limit);
-    p.few = !any ? 0 : (int)((most <= limit ? most : G) + 15) / 16 * 16;
+    const long long others = std::max(0, r.tokens - r.max_tokens), usual = (others + r.rows - 2) / std::max(1, r.rows - 1) * G;
+    p.few = !any ? 0 : (int)((most <= limit ? most : usual <= limit ? std::max<long long>(usual, G) : G) + 15) / 16 * 16;
     p.target = PAGED_PER_CU * q38_device_cus();
     const long long heads = (long long)r.rows * c.kv_heads, units = ((long long)r.max_pages * c.page_size + r.max_tokens + 63) / 64 / 4 + 2;
     p.joins = (int)std::min<long long>(most, p.few);

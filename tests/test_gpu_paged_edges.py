@@ -160,6 +160,17 @@ def test_many_rows(gpu, hd, hq, hkv):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hd, hq, hkv", [(64, 6, 1), (128, 8, 2), (256, 12, 2)])
+@pytest.mark.parametrize("lengths", [[4, 4, 200, 4, 4], [4, 90, 7, 1, 0, 8], [1, 1, 1, 100], [10, 11, 12, 100], [100, 4, 30, 30]])
+def test_rows_of_a_few_tokens_beside_a_long_one(gpu, hd, hq, hkv, lengths):
+    """The rows that stream are chosen by the others' usual number of tokens: some fit, some do not."""
+    args, call, want = attend_case(hq, hkv, hd, 32, lengths, [(97 * r) % 700 for r in range(len(lengths))], {})
+    check_attention(ext.paged_attention(*args, **call), want)
+    more = {**call, "max_tokens": sum(lengths)}  # a bound that no row comes near
+    check_attention(ext.paged_attention(*args, **more), want)
+
+
+@pytest.mark.gpu
 def test_many_rows_of_one_token_and_a_long_row(gpu):
     args, call, want = attend_case(2, 1, 64, 128, [1] * 200, [(37 * r) % 3000 for r in range(200)], {})
     check_attention(ext.paged_attention(*args, **call), want)
