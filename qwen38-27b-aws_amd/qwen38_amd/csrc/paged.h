@@ -25,7 +25,7 @@ struct PagedPlan {
     int few;                 // rows with at most this many (token, query head) pairs per KV head stream their positions, 16 pairs a tile
     int target;              // workgroups that their positions are cut into, about
     int items, slots, joins;  // workgroups of those at most; of them those that leave partial sums; pairs of a row at most
-    int tiles, parts, cus;   // workgroups of tiles of query rows; parts that few tiles' work is cut into (0: they are many); CUs
+    int tiles, parts, cus;   // workgroups of tiles of query rows; parts that few tiles' work is cut into (0: they are many); the device's CUs
     size_t table, part, cuts, cut_part, bytes;  // places in the scratch: the (row, KV head)s' first slot and count and their partial
                                                 // sums; the number of parts, the PagedCuts of them 256 bytes on, their sums; its size
 };

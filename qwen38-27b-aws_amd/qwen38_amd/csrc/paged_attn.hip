@@ -99,16 +99,23 @@ __device__ __forceinline__ void paged_scores(const PagedAttnArgs& a, float (&s)[
 //
 // Bound: the cache's bytes from memory. With one tile of query rows two waves share a SIMD, with a tile's loads in flight each (16
 // or 32 KB); with more, the sums and the queries mostly take the whole register file, and one wave is left. 64 rows of 8,192 positions, 4 KV
-// heads of 256 and six query heads to each: 187 us, 5.0 TB/s; 16 rows of 4 tokens after 32,768: 210 us, 4.5 TB/s; one row of 262,144
-// positions, 8 heads of 128: 116 us, 4.6 TB/s. Blocks of 16 positions per lane group (PT) where the registers hold them,
+// heads of 256 and six query heads to each: 187 us, 5.0 TB/s; 16 rows of 4 tokens after 32,768: 187 us, 5.1 TB/s; one row of 262,144
+// positions, 8 heads of 128: 100 us, 5.4 TB/s. Blocks of 16 positions per lane group (PT) where the registers hold them,
 // 8 for heads of 256: with 16 those spilled (decode 197 us, verify 237).
 //
-// The work is cut on the device, where the lengths are: units of 256 positions (a tile for each wave) of every row and KV head, as
-// many per workgroup as give PAGED_PER_CU workgroups per CU, rows in order. A (row, KV head) that one workgroup has all of is written
+// The work is cut on the device, where the lengths are: units of 256 positions (a tile or two for each wave) of every row and KV head, as
+// many per workgroup as give PAGED_PER_CU workgroups per CU, but PAGED_LEAST of them while the CUs have one each, rows in order. A (row, KV head) that one workgroup has all of is written
 // out by it; the others' sums go to scratch slots, which paged_join_kernel puts together.
 namespace {
 
-constexpr int PAGED_PER_CU = 4;  // workgroups that the work is cut into, per CU
+// Workgroups that the work is cut into, per CU. Each begins with a few loads one after another (its place in the work, queries, first
+// pages) and ends with its sums; more of them even out the CUs. us with 1, 2, 3, 4 per CU: one tile of query rows, heads of 256, 64 rows of 8,192
+// positions 220, 194, 187, 184, 16 of 16,384 120, 94, 94, 97, one of 262,144 101, 104, 110, 119; heads of 128, 64 rows of 8,192
+// 171, 191, 177, 180, one of 262,144 100, 101, 104, 110; two tiles, heads of 256, 16 rows of 4 after 32,768 267, 187, 197, 210; three
+// and more 16 rows after 32,768, heads of 128 170, 153, -, 141, of 256 -, 373, -, 322.
+constexpr int PAGED_PER_CU(int hd, int tiles) { return tiles > 2 ? 4 : tiles == 2 ? 2 : hd > 128 ? 3 : 1; }
+// 64 rows of 4 tokens after 512 positions, heads of 256: 28 us, with a unit each 51; one token each 19 and 25.
+constexpr int PAGED_LEAST = 3;
 
 struct PagedItem {
     int row, kvh, chunk, chunks, slot;  // slot: the item's place among the partial sums, -1 if it has its (row, KV head) whole
@@ -123,14 +130,16 @@ __device__ __forceinline__ int paged_units(const PagedAttnArgs& a, int row, int 
     return max(1, ((r.p0 + r.n + 63) / 64 - lo + 3) / 4);
 }
 
-__device__ __forceinline__ bool paged_item(const PagedAttnArgs& a, int id, int G, int target, PagedItem& it) {
+__device__ __forceinline__ bool paged_item(const PagedAttnArgs& a, int id, int G, PagedItem& it) {
     const int lane = threadIdx.x & 63, Hkv = a.c.kv_heads;
     const int units0 = lane < a.r.rows ? paged_units(a, lane, G) : 0;  // of the first 64 rows, for both rounds
     double total = units0;
     for (int row = lane + 64; row < a.r.rows; row += 64) total += paged_units(a, row, G);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
-    const int per = max(1, (int)((total * Hkv + (target - 1)) / target));
+    total *= Hkv;
+    const int target = a.plan.target, cus = a.plan.cus;
+    const int per = max(max(1, (int)((total + (target - 1)) / target)), min(PAGED_LEAST, (int)((total + (cus - 1)) / cus)));
     int before = 0, slots = 0;  // items and slots of the rows so far
     for (int base = 0; base < a.r.rows; base += 64) {
         const int row = base + lane;
@@ -169,7 +178,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PAGED_WAVES
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
     const int Hkv = a.c.kv_heads, G = a.q_heads / Hkv, ps = a.c.page_size, shift = __builtin_ctz(ps);
     PagedItem it;
-    if (!paged_item(a, blockIdx.x, G, a.plan.target, it)) return;
+    if (!paged_item(a, blockIdx.x, G, it)) return;
     it = {uniform(it.row), uniform(it.kvh), uniform(it.chunk), uniform(it.chunks), uniform(it.slot)};
     const PagedRow r = paged_row_uniform(a.r, it.row, ps);
     const int R = r.n * G, total = r.p0 + r.n;
@@ -899,7 +908,8 @@ PagedPlan paged_attention_plan(const PagedCache& c, const PagedRows& r, int q_he
     const bool any = most <= limit || (r.q_start && G <= limit);
     const long long others = std::max(0, r.tokens - r.max_tokens), usual = (others + r.rows - 2) / std::max(1, r.rows - 1) * G;
     p.few = !any ? 0 : (int)((most <= limit ? most : usual <= limit ? std::max<long long>(usual, G) : G) + 15) / 16 * 16;
-    p.target = PAGED_PER_CU * q38_device_cus();
+    p.cus = q38_device_cus();
+    p.target = PAGED_PER_CU(c.head_dim, p.few / 16) * p.cus;
     const long long heads = (long long)r.rows * c.kv_heads, units = ((long long)r.max_pages * c.page_size + r.max_tokens + 63) / 64 / 4 + 2;
     p.joins = (int)std::min<long long>(most, p.few);
     p.items = any ? (int)std::min<long long>(p.target + heads, heads * units) : 0;
@@ -912,7 +922,6 @@ PagedPlan paged_attention_plan(const PagedCache& c, const PagedRows& r, int q_he
     }
     if (most > p.few) {
         const long long jobs = heads * ((most + PT_TILE - 1) / PT_TILE);
-        p.cus = q38_device_cus();
         const long long blocks = ((long long)r.max_pages * c.page_size + r.max_tokens + 31) / 32 + 1;
         const bool many = jobs >= (long long)PT_FEW * p.cus;
         p.parts = many && !r.q_start ? 0 : (int)std::min<long long>(p.cus * PT_PER_CU(c.head_dim), std::max<long long>(1, jobs * blocks / PT_LEAST));
@@ -953,7 +962,7 @@ hipError_t q38_paged_attention(const PagedAttnArgs& a, hipStream_t stream) {
         const int heads = a.r.rows * a.c.kv_heads;
 #define JOIN(E)                                                                                                              \
     do {                                                                                                                     \
-        if (heads * 32 <= a.plan.target)                                                                                     \
+        if (heads * 8 <= a.plan.cus)                                                                                         \
             hipLaunchKernelGGL((paged_join_kernel<E, 16>), dim3(heads * a.plan.joins), dim3(1024), 0, stream, a);            \
         else                                                                                                                 \
             hipLaunchKernelGGL((paged_join_kernel<E, 4>), dim3(heads * a.plan.joins), dim3(256), 0, stream, a);              \
