@@ -99,7 +99,7 @@ __device__ __forceinline__ void paged_scores(const PagedAttnArgs& a, float (&s)[
 //
 // Bound: the cache's bytes from memory. With one tile of query rows two waves share a SIMD, with a tile's loads in flight each (16
 // or 32 KB); with more, the sums and the queries mostly take the whole register file, and one wave is left. 64 rows of 8,192 positions, 4 KV
-// heads of 256 and six query heads to each: 187 us, 5.0 TB/s; 16 rows of 4 tokens after 32,768: 187 us, 5.1 TB/s; one row of 262,144
+// heads of 256 and six query heads to each: 187 to 190 us, 5.0 TB/s; 16 rows of 4 tokens after 32,768: 187 us, 5.1 TB/s; one row of 262,144
 // positions, 8 heads of 128: 100 us, 5.4 TB/s. Blocks of 16 positions per lane group (PT) where the registers hold them,
 // 8 for heads of 256: with 16 those spilled (decode 197 us, verify 237).
 //
