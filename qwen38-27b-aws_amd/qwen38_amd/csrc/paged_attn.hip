@@ -476,7 +476,9 @@ constexpr int PT_TILE = 256;
 constexpr int PT_FEW = 3;  // tiles per CU: with as many they go whole, a workgroup each
 // Sub-blocks of a part. Beginning a tile costs some 15,000 clocks (its work found, its first pages and queries read), as much as
 // five sub-blocks of heads of 128: 777 tokens after none in parts of 12 took 78 us, of 8 (more of them) 59, whole 46.
-constexpr int PT_LEAST = 16;
+// Of heads of 64 a sub-block takes half as long, but two workgroups begin beside each other: parts of 8 (4 prompts of 624 to 1,000 with
+// slopes 71 us against 74, 777 tokens after none 31 against 37).
+constexpr int PT_LEAST(int head_dim) { return head_dim > 64 ? 16 : 8; }
 constexpr int PT_PER_CU(int head_dim) { return head_dim > 64 ? 1 : 2; }  // workgroups that a CU holds
 __device__ __forceinline__ v8bf16 paged_frag(uint32_t at) {
     return *(const __attribute__((address_space(3))) v8bf16*)(uintptr_t)at;
@@ -582,8 +584,8 @@ __device__ __forceinline__ PagedWork paged_work(const PagedAttnArgs& a, int G) {
     const PagedJob all = paged_tiles_list(a, G, false, 0, false);
     const int jobs = all.tile * a.c.kv_heads;
     const long long total = all.start * a.c.kv_heads;
-    if (!a.plan.parts || jobs >= PT_FEW * a.plan.cus || all.units <= 2 * PT_LEAST) return {jobs, jobs, jobs, true, 1, 0};
-    const int parts = (int)max(1LL, min((long long)a.plan.parts, total / PT_LEAST));
+    if (!a.plan.parts || jobs >= PT_FEW * a.plan.cus || all.units <= 2 * PT_LEAST(a.c.head_dim)) return {jobs, jobs, jobs, true, 1, 0};
+    const int parts = (int)max(1LL, min((long long)a.plan.parts, total / PT_LEAST(a.c.head_dim)));
     const long long each = quotient(total, parts);
     return {total, jobs, parts, false, each, total - each * parts};
 }
@@ -924,7 +926,7 @@ PagedPlan paged_attention_plan(const PagedCache& c, const PagedRows& r, int q_he
         const long long jobs = heads * ((most + PT_TILE - 1) / PT_TILE);
         const long long blocks = ((long long)r.max_pages * c.page_size + r.max_tokens + 31) / 32 + 1;
         const bool many = jobs >= (long long)PT_FEW * p.cus;
-        p.parts = many && !r.q_start ? 0 : (int)std::min<long long>(p.cus * PT_PER_CU(c.head_dim), std::max<long long>(1, jobs * blocks / PT_LEAST));
+        p.parts = many && !r.q_start ? 0 : (int)std::min<long long>(p.cus * PT_PER_CU(c.head_dim), std::max<long long>(1, jobs * blocks / PT_LEAST(c.head_dim)));
         p.tiles = (int)std::max<long long>(p.parts, jobs);
         if (p.parts) {
             p.cuts = p.bytes + 255 & ~(size_t)255;
