@@ -405,11 +405,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PAGED_WAVES
 // four waves), four where they are few and the workgroups many (64 rows of 8,192 positions: 189 us in all against 204 with
 // sixteen).
 template <int E, int W>
-__global__ __launch_bounds__(W * 64) void paged_join_kernel(const PagedAttnArgs a) {
+__device__ __forceinline__ void paged_join(const PagedAttnArgs& a, int block) {
     constexpr int HD = E * 64;
     __shared__ float sums[W][HD], totals[W];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, Hkv = a.c.kv_heads, G = a.q_heads / Hkv;
-    const int n = a.plan.joins, q = blockIdx.x % n, kvh = blockIdx.x / n % Hkv, row = blockIdx.x / n / Hkv;
+    const int n = a.plan.joins, q = block % n, kvh = block / n % Hkv, row = block / n / Hkv;
     const PagedRow r = paged_row(a.r, row, a.c.page_size);
     if (q >= r.n * G || r.n * G > a.plan.few) return;
     const int2 t = ((const int2*)(a.scratch + a.plan.table))[row * Hkv + kvh];
@@ -451,6 +451,11 @@ __global__ __launch_bounds__(W * 64) void paged_join_kernel(const PagedAttnArgs 
         for (int w = 0; w < W; ++w) all += totals[w], x += sums[w][d];
         out[d] = f2bf(x / all);
     }
+}
+
+template <int E, int W>
+__global__ __launch_bounds__(W * 64) void paged_join_kernel(const PagedAttnArgs a) {
+    paged_join<E, W>(a, blockIdx.x);
 }
 
 // ---- Many query rows (prefill chunks): tiles of 256 query rows (tokens x the KV head's query heads) per workgroup.
@@ -510,7 +515,7 @@ __device__ __forceinline__ long long quotient(long long a, long long b) {
 struct PagedWork {
     long long total;
     int jobs, parts;
-    bool whole;
+    bool whole, kept;
     long long each, longer;  // units of a part; the first `longer` have one more
     __device__ __forceinline__ long long start(int w) const { return each * w + min((long long)w, longer); }
     __device__ __forceinline__ int part(long long u) const {  // that unit u is in
@@ -532,8 +537,10 @@ __device__ __forceinline__ long long uniform(long long x) {
 
 // Goes over the tiles, a lane for each: 64 rows' numbers of tiles at a time, then 64 of their tiles, whose rows the lanes look up among
 // them. Without `find` it returns the work's total of sub-blocks per KV head, number of tiles and longest tile in job.start, tile and units; with it
-// the job of unit u.
-__device__ __forceinline__ PagedJob paged_tiles_list(const PagedAttnArgs& a, int G, bool find, long long u, bool whole) {
+// the job of unit u. `keep` receives the lanes' first tiles.
+typedef int PagedKept[4][64];  // sub-blocks up to the tile's end, its own, its row, its place in the row
+
+__device__ __forceinline__ PagedJob paged_tiles_list(const PagedAttnArgs& a, int G, bool find, long long u, bool whole, PagedKept* keep) {
     const int lane = threadIdx.x & 63, Hkv = a.c.kv_heads;
     long long before = 0;
     int tiles = 0, longest = 1;
@@ -559,6 +566,12 @@ __device__ __forceinline__ PagedJob paged_tiles_list(const PagedAttnArgs& a, int
             const int units = k >= count ? 0 : whole ? 1 : max(1, s.hi - s.lo);
             longest = max(longest, units);
             const uint32_t sum = lanes_up_to(units);  // of 64 tiles of up to 2^25 sub-blocks and a token's
+            if (keep && base == 0 && k0 == 0 && threadIdx.x < 64) {
+                (*keep)[0][lane] = (int)sum;
+                (*keep)[1][lane] = units;
+                (*keep)[2][lane] = l;
+                (*keep)[3][lane] = tile;
+            }
             const unsigned long long past = find ? __ballot(before + (long long)sum * Hkv > u) : 0;
             if (past) {
                 const int f = __ffsll(past) - 1;
@@ -580,14 +593,32 @@ __device__ __forceinline__ PagedJob paged_tiles_list(const PagedAttnArgs& a, int
     return {-1, tiles, 0, before, uniform(longest)};
 }
 
-__device__ __forceinline__ PagedWork paged_work(const PagedAttnArgs& a, int G) {
-    const PagedJob all = paged_tiles_list(a, G, false, 0, false);
+// The job of unit u: from the kept tiles where those are all (looking it up again takes 4,000 clocks of each tile), or from the list.
+// Not for heads of 256: the registers that this takes push others out of the loop (a prompt's chunk 855 us against 805).
+__device__ __forceinline__ PagedJob paged_tiles_find(const PagedAttnArgs& a, int G, long long u, bool whole, bool kept, const PagedKept& keep) {
+    if (!kept) return paged_tiles_list(a, G, true, u, whole, nullptr);
+    const int lane = threadIdx.x & 63, Hkv = a.c.kv_heads, units = keep[1][lane];
+    const uint32_t sum = keep[0][lane];
+    const int f = whole ? (int)u / Hkv : __ffsll((unsigned long long)__ballot((long long)sum * Hkv > u)) - 1;
+    PagedJob job;
+    job.row = lane_of(keep[2][lane], f);
+    job.tile = lane_of(keep[3][lane], f);
+    job.units = whole ? 1 : lane_of(units, f);
+    const long long first = whole ? (long long)f * Hkv : (long long)(uint32_t)lane_of(sum - units, f) * Hkv;
+    job.kvh = (int)quotient(u - first, job.units);
+    job.start = first + (long long)job.kvh * job.units;
+    return job;
+}
+
+__device__ __forceinline__ PagedWork paged_work(const PagedAttnArgs& a, int G, PagedKept* keep) {
+    const PagedJob all = paged_tiles_list(a, G, false, 0, false, keep);
     const int jobs = all.tile * a.c.kv_heads;
     const long long total = all.start * a.c.kv_heads;
-    if (!a.plan.parts || jobs >= PT_FEW * a.plan.cus || all.units <= 2 * PT_LEAST(a.c.head_dim)) return {jobs, jobs, jobs, true, 1, 0};
+    const bool kept = keep && a.r.rows <= 64 && all.tile <= 64;
+    if (!a.plan.parts || jobs >= PT_FEW * a.plan.cus || all.units <= 2 * PT_LEAST(a.c.head_dim)) return {jobs, jobs, jobs, true, kept, 1, 0};
     const int parts = (int)max(1LL, min((long long)a.plan.parts, total / PT_LEAST(a.c.head_dim)));
     const long long each = quotient(total, parts);
-    return {total, jobs, parts, false, each, total - each * parts};
+    return {total, jobs, parts, false, kept, each, total - each * parts};
 }
 
 // A cut tile in the scratch's table, at the workgroup that begins it: which workgroups' sums make it.
@@ -609,13 +640,16 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2 * PT_PER_
     __shared__ float slopes[PT_TILE];
     const int lane = threadIdx.x & 63, wv = uniform((int)threadIdx.x >> 6), l32 = lane & 31, h = lane >> 5;
     const int Hkv = a.c.kv_heads, G = a.q_heads / Hkv, ps = a.c.page_size, shift = __builtin_ctz(ps);
-    const PagedWork work = paged_work(a, G);
+    constexpr bool KEEP = HD <= 128;
+    __shared__ PagedKept keep;
+    const PagedWork work = paged_work(a, G, KEEP ? &keep : nullptr);
     const int w = blockIdx.x;
     if (w == 0 && threadIdx.x == 0 && a.plan.parts) *(int*)(a.scratch + a.plan.cuts) = work.whole || !work.jobs ? 0 : work.parts;
     if (!work.jobs || w >= work.parts) return;
+    if constexpr (KEEP) __syncthreads();
     const long long begin = work.start(w), end = work.start(w + 1);
     for (long long unit = begin; unit < end;) {
-    const PagedJob job = paged_tiles_list(a, G, true, unit, work.whole);
+    const PagedJob job = paged_tiles_find(a, G, unit, work.whole, KEEP && work.kept, keep);
     if (job.row < 0) return;
     const PagedRow r = paged_row_uniform(a.r, job.row, ps);
     const int R = r.n * G, total = r.p0 + r.n, prefix = a.prefix ? uniform(a.prefix[job.row]) : 0;
@@ -867,13 +901,15 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2 * PT_PER_
     }
 }
 
-// The parts of cut tiles put together. Grid: parts (the tile that each begins, if it is cut) x the tile's eight groups of 32 query rows x dims in blocks of 32.
+// The parts of cut tiles put together. Grid: parts (the tile that each begins, if it is cut) x the tile's eight groups of 32 query
+// rows x dims in blocks of 32; behind those of the rows that streamed, if some may have been cut: one launch for both.
 template <int HD>
-__global__ __launch_bounds__(256) void paged_join_tiles_kernel(const PagedAttnArgs a) {
+__global__ __launch_bounds__(256) void paged_join_tiles_kernel(const PagedAttnArgs a, int streamed) {
+    if ((int)blockIdx.x < streamed) return paged_join<HD / 64, 4>(a, blockIdx.x);
     constexpr int VD = HD / 32;
     const int lane = threadIdx.x & 63, q = threadIdx.x >> 6, l32 = lane & 31, h = lane >> 5;
-    const int Hkv = a.c.kv_heads, G = a.q_heads / Hkv;
-    const int d = blockIdx.x % VD, group = blockIdx.x / VD % 8, j = blockIdx.x / VD / 8;
+    const int Hkv = a.c.kv_heads, G = a.q_heads / Hkv, block = blockIdx.x - streamed;
+    const int d = block % VD, group = block / VD % 8, j = block / VD / 8;
     if (j >= *(const int*)(a.scratch + a.plan.cuts)) return;
     const PagedCut job = ((const PagedCut*)(a.scratch + a.plan.cuts + 256))[j];
     if (job.first == job.last) return;
@@ -944,6 +980,7 @@ bool paged_attention_fits(const PagedCache& c, const PagedRows& r, int q_heads) 
 
 hipError_t q38_paged_attention(const PagedAttnArgs& a, hipStream_t stream) {
     const int few = a.plan.few, G = a.q_heads / a.c.kv_heads;
+    int joins = 0;
     if (a.plan.items) {
 #define STREAM(HD, NT) hipLaunchKernelGGL((paged_stream_kernel<HD, NT, (HD > 128 ? 8 : 16)>), dim3(a.plan.items), dim3(256), 0, stream, a)
         switch (a.c.head_dim * 8 + few / 16) {
@@ -962,25 +999,29 @@ hipError_t q38_paged_attention(const PagedAttnArgs& a, hipStream_t stream) {
         }
 #undef STREAM
         const int heads = a.r.rows * a.c.kv_heads;
+        joins = a.plan.slots ? heads * a.plan.joins : 0;
+        if ((long long)a.r.max_tokens * G <= few) {
 #define JOIN(E)                                                                                                              \
     do {                                                                                                                     \
         if (heads * 8 <= a.plan.cus)                                                                                         \
-            hipLaunchKernelGGL((paged_join_kernel<E, 16>), dim3(heads * a.plan.joins), dim3(1024), 0, stream, a);            \
+            hipLaunchKernelGGL((paged_join_kernel<E, 16>), dim3(joins), dim3(1024), 0, stream, a);                           \
         else                                                                                                                 \
-            hipLaunchKernelGGL((paged_join_kernel<E, 4>), dim3(heads * a.plan.joins), dim3(256), 0, stream, a);              \
+            hipLaunchKernelGGL((paged_join_kernel<E, 4>), dim3(joins), dim3(256), 0, stream, a);                             \
     } while (0)
-        switch (a.plan.slots ? a.c.head_dim : 0) {
-            case 64: JOIN(1); break;
-            case 128: JOIN(2); break;
-            case 256: JOIN(4); break;
-        }
+            switch (joins ? a.c.head_dim : 0) {
+                case 64: JOIN(1); break;
+                case 128: JOIN(2); break;
+                case 256: JOIN(4); break;
+            }
 #undef JOIN
-        if ((long long)a.r.max_tokens * G <= few) return hipGetLastError();
+            return hipGetLastError();
+        }
     }
 #define TILES(HD)                                                                                                             \
     do {                                                                                                                     \
         hipLaunchKernelGGL((paged_tiles_kernel<HD>), dim3(a.plan.tiles), dim3(512), 0, stream, a);                           \
-        if (a.plan.parts) hipLaunchKernelGGL((paged_join_tiles_kernel<HD>), dim3(a.plan.parts * 8 * (HD / 32)), dim3(256), 0, stream, a); \
+        if (joins || a.plan.parts)                                                                                           \
+            hipLaunchKernelGGL((paged_join_tiles_kernel<HD>), dim3(joins + a.plan.parts * 8 * (HD / 32)), dim3(256), 0, stream, a, joins); \
     } while (0)
     switch (a.c.head_dim) {
         case 64: TILES(64); break;
