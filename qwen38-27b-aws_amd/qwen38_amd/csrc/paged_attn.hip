@@ -959,7 +959,9 @@ PagedPlan paged_attention_plan(const PagedCache& c, const PagedRows& r, int q_he
         p.bytes = p.part + (size_t)p.slots * p.few * (c.head_dim + 2) * 4;
     }
     if (most > p.few) {
-        const long long jobs = heads * ((most + PT_TILE - 1) / PT_TILE);
+        // Of a ragged call's tokens at most so many tiles (a workgroup that finds no work still takes its turn on a CU: 24 rows, one of
+        // 777 tokens, 155 us with a workgroup for as many in each row).
+        const long long jobs = std::min(heads * ((most + PT_TILE - 1) / PT_TILE), c.kv_heads * ((long long)r.tokens * G / PT_TILE + r.rows));
         const long long blocks = ((long long)r.max_pages * c.page_size + r.max_tokens + 31) / 32 + 1;
         const bool many = jobs >= (long long)PT_FEW * p.cus;
         p.parts = many && !r.q_start ? 0 : (int)std::min<long long>(p.cus * PT_PER_CU(c.head_dim), std::max<long long>(1, jobs * blocks / PT_LEAST(c.head_dim)));
