@@ -118,7 +118,7 @@ constexpr int append_room(int head_dim, int nw, int steps) { return nw * (64 / (
 // Grid: per row, page it may touch and KV head one workgroup; then the queries, QUERY_STEPS vectors per lane. A workgroup has all
 // of its page's new tokens, so the page's largest value is known before any of them is coded, and every input is read once.
 // Bound: memory; for a few tokens a launch's and four loads' time, one after another. With 24 query and 4 KV heads of 256: one token
-// 5.8 us, 64 rows of 4 tokens 7.7, 2,048 tokens of a prompt 19 (3.3 TB/s); 37 prompts, 32 and 8 heads of 128, pages of 16, 80 us (5.2 TB/s).
+// 4.4 us, 64 rows of 4 tokens 5.9, 2,048 tokens of a prompt 17 (3.7 TB/s); 37 prompts, 32 and 8 heads of 128, pages of 16, 77 us (5.4 TB/s).
 template <int HD, int NW, int STEPS>
 __global__ __launch_bounds__(NW * 64) void paged_append_kernel(const PagedAppendArgs a) {
     constexpr int VECS = 64 / (HD / 8);  // vectors of a wave at a time

@@ -99,8 +99,8 @@ __device__ __forceinline__ void paged_scores(const PagedAttnArgs& a, float (&s)[
 //
 // Bound: the cache's bytes from memory. With one tile of query rows two waves share a SIMD, with a tile's loads in flight each (16
 // or 32 KB); with more, the sums and the queries mostly take the whole register file, and one wave is left. 64 rows of 8,192 positions, 4 KV
-// heads of 256 and six query heads to each: 187 to 190 us, 5.0 TB/s; 16 rows of 4 tokens after 32,768: 187 us, 5.1 TB/s; one row of 262,144
-// positions, 8 heads of 128: 100 us, 5.4 TB/s. Blocks of 16 positions per lane group (PT) where the registers hold them,
+// heads of 256 and six query heads to each: 181 us, 5.2 TB/s; 16 rows of 4 tokens after 32,768: 186 us, 5.1 TB/s; one row of 262,144
+// positions, 8 heads of 128: 97 us, 5.5 TB/s. Blocks of 16 positions per lane group (PT) where the registers hold them,
 // 8 for heads of 256: with 16 those spilled (decode 197 us, verify 237).
 //
 // The work is cut on the device, where the lengths are: units of 256 positions (a tile or two for each wave) of every row and KV head, as
@@ -109,10 +109,10 @@ __device__ __forceinline__ void paged_scores(const PagedAttnArgs& a, float (&s)[
 namespace {
 
 // Workgroups that the work is cut into, per CU. Each begins with a few loads one after another (its place in the work, queries, first
-// pages) and ends with its sums; more of them even out the CUs. us with 1, 2, 3, 4 per CU: one tile of query rows, heads of 256, 64 rows of 8,192
-// positions 220, 194, 187, 184, 16 of 16,384 120, 94, 94, 97, one of 262,144 101, 104, 110, 119; heads of 128, 64 rows of 8,192
-// 171, 191, 177, 180, one of 262,144 100, 101, 104, 110; two tiles, heads of 256, 16 rows of 4 after 32,768 267, 187, 197, 210; three
-// and more 16 rows after 32,768, heads of 128 170, 153, -, 141, of 256 -, 373, -, 322.
+// pages) and ends with its sums; more of them even out the CUs. One tile of query rows, heads of 256: 64 rows of 8,192 positions 188,
+// 181 and 176 us with 2, 3 and 4, 16 of 16,384 91, 92 and 98, one of 262,144 98, 102 and 114; heads of 128: 64 rows of 8,192 164 and 196
+// with 1 and 2, one of 262,144 97 and 101. Two tiles, heads of 256, 16 rows of 4 after 32,768: 186 and 201 with 2 and 3. Three
+// tiles, 16 rows after 32,768, heads of 256 356 and 312 with 2 and 4, of 128 159 and 146.
 constexpr int PAGED_PER_CU(int hd, int tiles) { return tiles > 2 ? 4 : tiles == 2 ? 2 : hd > 128 ? 3 : 1; }
 // 64 rows of 4 tokens after 512 positions, heads of 256: 28 us, with a unit each 51; one token each 19 and 25.
 constexpr int PAGED_LEAST = 3;
