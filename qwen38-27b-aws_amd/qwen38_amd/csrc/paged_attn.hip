@@ -475,8 +475,8 @@ __global__ __launch_bounds__(W * 64) void paged_join_kernel(const PagedAttnArgs 
 // which 1,024; of heads of 64, whose registers let two workgroups share a CU, 1,300 of 512. Four waves of 64 rows read LDS half
 // as often, but have no second wave to fill a SIMD's pauses: 0.83 ms.
 //
-// While tiles are few, the sub-blocks of 32 positions of all of them, one after another, are dealt out to the CUs in equal
-// parts: a workgroup ends one tile, takes some whole and begins another. What it has of a tile that others share goes to scratch
+// While tiles are few, the sub-blocks of 32 positions of all of them, one after another, and the beginning of each, are dealt out to
+// the CUs in equal parts: a workgroup ends one tile, takes some whole and begins another. What it has of a tile that others share goes to scratch
 // in float32 (256 KB for heads of 256, a dozen sub-blocks' time), and paged_join_tiles_kernel puts it together.
 namespace {
 
@@ -487,6 +487,10 @@ constexpr int PT_FEW = 3;  // tiles per CU: with as many they go whole, a workgr
 // Of heads of 64 a sub-block takes half as long, but two workgroups begin beside each other: parts of 8 (4 prompts of 624 to 1,000 with
 // slopes 71 us against 74, 777 tokens after none 31 against 37).
 constexpr int PT_LEAST(int head_dim) { return head_dim > 64 ? 16 : 8; }
+// What beginning a tile counts as, in sub-blocks (fewer than a part has); a part that would end within it leaves the tile to the next. 4
+// prompts with slopes 62 us, counting nothing 66; 777 tokens after 4,000 59 and 66. For larger heads, whose sub-blocks take
+// longer, nothing: what it saves there (2% of short calls) their loops lose by the registers that it takes.
+constexpr int PT_START(int head_dim) { return head_dim > 64 ? 0 : 7; }
 constexpr int PT_PER_CU(int head_dim) { return head_dim > 64 ? 1 : 2; }  // workgroups that a CU holds
 __device__ __forceinline__ v8bf16 paged_frag(uint32_t at) {
     return *(const __attribute__((address_space(3))) v8bf16*)(uintptr_t)at;
@@ -543,6 +547,7 @@ __device__ __forceinline__ long long uniform(long long x) {
 // the job of unit u. `keep` receives the lanes' first tiles.
 typedef int PagedKept[4][64];  // sub-blocks up to the tile's end, its own, its row, its place in the row
 
+template <int HD>
 __device__ __forceinline__ PagedJob paged_tiles_list(const PagedAttnArgs& a, int G, bool find, long long u, bool whole, PagedKept* keep) {
     const int lane = threadIdx.x & 63, Hkv = a.c.kv_heads;
     long long before = 0;
@@ -566,7 +571,7 @@ __device__ __forceinline__ PagedJob paged_tiles_list(const PagedAttnArgs& a, int
             mine.t0 = 0;
             const int tile = __shfl(ends, l) - 1 - k;  // the latest tokens, the longest tiles, first
             const PagedSpan s = paged_span(a, mine, __shfl(prefix, l), max(tile, 0), G);
-            const int units = k >= count ? 0 : whole ? 1 : max(1, s.hi - s.lo);
+            const int units = k >= count ? 0 : whole ? 1 : max(1, s.hi - s.lo) + PT_START(HD);
             longest = max(longest, units);
             const uint32_t sum = lanes_up_to(units);  // of 64 tiles of up to 2^25 sub-blocks and a token's
             if (keep && base == 0 && k0 == 0 && threadIdx.x < 64) {
@@ -598,8 +603,9 @@ __device__ __forceinline__ PagedJob paged_tiles_list(const PagedAttnArgs& a, int
 
 // The job of unit u: from the kept tiles where those are all (looking it up again takes 4,000 clocks of each tile), or from the list.
 // Not for heads of 256: the registers that this takes push others out of the loop (a prompt's chunk 855 us against 805).
+template <int HD>
 __device__ __forceinline__ PagedJob paged_tiles_find(const PagedAttnArgs& a, int G, long long u, bool whole, bool kept, const PagedKept& keep) {
-    if (!kept) return paged_tiles_list(a, G, true, u, whole, nullptr);
+    if (!kept) return paged_tiles_list<HD>(a, G, true, u, whole, nullptr);
     const int lane = threadIdx.x & 63, Hkv = a.c.kv_heads, units = keep[1][lane];
     const uint32_t sum = keep[0][lane];
     const int f = whole ? (int)u / Hkv : __ffsll((unsigned long long)__ballot((long long)sum * Hkv > u)) - 1;
@@ -613,13 +619,14 @@ __device__ __forceinline__ PagedJob paged_tiles_find(const PagedAttnArgs& a, int
     return job;
 }
 
+template <int HD>
 __device__ __forceinline__ PagedWork paged_work(const PagedAttnArgs& a, int G, PagedKept* keep) {
-    const PagedJob all = paged_tiles_list(a, G, false, 0, false, keep);
+    const PagedJob all = paged_tiles_list<HD>(a, G, false, 0, false, keep);
     const int jobs = all.tile * a.c.kv_heads;
     const long long total = all.start * a.c.kv_heads;
     const bool kept = keep && a.r.rows <= 64 && all.tile <= 64;
-    if (!a.plan.parts || jobs >= PT_FEW * a.plan.cus || all.units <= 2 * PT_LEAST(a.c.head_dim)) return {jobs, jobs, jobs, true, kept, 1, 0};
-    const int parts = (int)max(1LL, min((long long)a.plan.parts, total / PT_LEAST(a.c.head_dim)));
+    if (!a.plan.parts || jobs >= PT_FEW * a.plan.cus || all.units <= 2 * PT_LEAST(HD) + PT_START(HD)) return {jobs, jobs, jobs, true, kept, 1, 0};
+    const int parts = (int)max(1LL, min((long long)a.plan.parts, total / PT_LEAST(HD)));
     const long long each = quotient(total, parts);
     return {total, jobs, parts, false, kept, each, total - each * parts};
 }
@@ -645,14 +652,14 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2 * PT_PER_
     const int Hkv = a.c.kv_heads, G = a.q_heads / Hkv, ps = a.c.page_size, shift = __builtin_ctz(ps);
     constexpr bool KEEP = HD <= 128;
     __shared__ PagedKept keep;
-    const PagedWork work = paged_work(a, G, KEEP ? &keep : nullptr);
+    const PagedWork work = paged_work<HD>(a, G, KEEP ? &keep : nullptr);
     const int w = blockIdx.x;
     if (w == 0 && threadIdx.x == 0 && a.plan.parts) *(int*)(a.scratch + a.plan.cuts) = work.whole || !work.jobs ? 0 : work.parts;
     if (!work.jobs || w >= work.parts) return;
     if constexpr (KEEP) __syncthreads();
     const long long begin = work.start(w), end = work.start(w + 1);
     for (long long unit = begin; unit < end;) {
-    const PagedJob job = paged_tiles_find(a, G, unit, work.whole, KEEP && work.kept, keep);
+    const PagedJob job = paged_tiles_find<HD>(a, G, unit, work.whole, KEEP && work.kept, keep);
     if (job.row < 0) return;
     const PagedRow r = paged_row_uniform(a.r, job.row, ps);
     const int R = r.n * G, total = r.p0 + r.n, prefix = a.prefix ? uniform(a.prefix[job.row]) : 0;
@@ -661,12 +668,20 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2 * PT_PER_
     // This part's tiles of 32 positions of those that any of the workgroup's query rows sees.
     const PagedSpan span = paged_span(a, r, prefix, job.tile, G);
     const long long stop = min(end, job.start + job.units);
-    const int T0 = span.lo + (work.whole ? 0 : (int)(unit - job.start)), T1 = work.whole ? span.hi : min(span.hi, span.lo + (int)(stop - job.start));
-    const bool alone = unit == job.start && stop == job.start + job.units;
+    int begun = (int)(unit - job.start), ended = (int)(stop - job.start);
+    bool left = false;
+    if constexpr (PT_START(HD) > 0) {
+        begun = max(begun - PT_START(HD), 0);
+        ended -= PT_START(HD);
+        left = !work.whole && ended <= 0;
+    }
+    const int T0 = span.lo + (work.whole ? 0 : begun), T1 = work.whole ? span.hi : min(span.hi, span.lo + ended);
+    const bool first = PT_START(HD) ? work.whole || begun == 0 : unit == job.start, alone = first && stop == job.start + job.units;
     const int slot = 2 * w + (unit > begin);
     // The tile that this part begins and others end: this part's last, at most one.
     if (stop == end && !work.whole && threadIdx.x == 0)
-        ((PagedCut*)(a.scratch + a.plan.cuts + 256))[w] = {job.row, job.tile, job.kvh, slot, w, unit == job.start && !alone ? work.part(job.start + job.units - 1) : w};
+        ((PagedCut*)(a.scratch + a.plan.cuts + 256))[w] = {job.row, job.tile, job.kvh, slot, w, first && !alone && !left ? work.part(job.start + job.units - 1) : w};
+    if (left) return;
     unit = stop;
 
     // The wave's query rows, a lane's (and lane ^ 32's) one, as B operands.
