@@ -471,8 +471,8 @@ __global__ __launch_bounds__(W * 64) void paged_join_kernel(const PagedAttnArgs 
 // run beside the other's MFMAs.
 //
 // Bound: the matrix cores and the exponentials together. A tile of heads of 256 takes 4,100 to 4,500 clocks, of which its MFMAs
-// are 2,048 (2,048 tokens after 14,336, 24 and 4 heads of 256: 0.75 to 0.85 ms, 0.9 to 1.0 PFLOP/s); of heads of 128 some 2,850, of
-// which 1,024; of heads of 64, whose registers let two workgroups share a CU, 1,300 of 512. Four waves of 64 rows read LDS half
+// are 2,048 and its LDS reads 2,300 (2,048 tokens after 14,336, 24 and 4 heads of 256: 0.72 to 0.83 ms, 0.9 to 1.07 PFLOP/s); of heads
+// of 128 some 2,600, of which 1,024; of heads of 64, whose registers let two workgroups share a CU, 1,500 of 512. Four waves of 64 rows read LDS half
 // as often, but have no second wave to fill a SIMD's pauses: 0.83 ms.
 //
 // While tiles are few, the sub-blocks of 32 positions of all of them, one after another, and the beginning of each, are dealt out to

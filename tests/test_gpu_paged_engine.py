@@ -237,3 +237,54 @@ def test_what_an_engine_refuses(gpu, weights):
         slab.paged_cache(0)
     with pytest.raises(ValueError):
         slab.set_pages(0, [0])
+
+
+@pytest.mark.gpu
+def test_a_loaded_model_decodes_over_pages(gpu, weights):
+    """`runner.load` with kv_pages: a prompt prefilled in chunks and decoded greedily, its rows' pages given as they are needed, is the
+    engine's whose rows had all theirs from the start."""
+    from qwen38_amd import runner
+
+    cfg, values = weights
+    kw = dict(cfg=cfg, batch_size=B, max_seq_len=S, verify_tokens=1, chunk=CHUNK, weight_format="e4m3", kv_cache_format="fp8", kv_page_size=PAGE,
+              log=lambda m: None)
+    one, other = (runner.load(weights=((n, v) for n, v in values.items() if not n.startswith("mtp.")), kv_pages=B * EACH, **kw) for _ in range(2))
+    free = list(range(B * EACH))[::-1]
+    held = [[] for _ in range(B)]
+    for r in range(B):
+        other.engine.set_pages(r, [])
+
+    def grow(row, tokens):
+        while len(held[row]) * PAGE < tokens:
+            held[row].append(free.pop())
+        other.engine.set_pages(row, held[row])
+
+    prompt = torch.randint(0, cfg.vocab_size, (CHUNK + 9,), generator=torch.Generator().manual_seed(9)).tolist()
+    ids = []
+    for model in (one, other):
+        out = []
+        for start in (0, CHUNK):
+            part = prompt[start : start + CHUNK]
+            if model is other:
+                grow(1, start + len(part))
+            x = torch.zeros(1, CHUNK, cfg.hidden_size, dtype=BF16, device="cuda")
+            x[0, : len(part)] = values["embed_tokens"][part].cuda()
+            h = model.prefill(inputs_embeds=x, **prefill_inputs(cfg, 1, start, len(part), CHUNK, BF16))[:, len(part) - 1 : len(part)]
+        at = len(prompt)
+        for _ in range(PAGE + 2):
+            token = model.head.next_tokens(h.expand(B, -1, -1).contiguous())[1]
+            out.append(token)
+            if model is other:
+                grow(1, at + 1)
+            x = values["embed_tokens"][[token]].cuda().expand(B, -1).unsqueeze(1).contiguous()
+            h = model.step(inputs_embeds=x, **batch_step_inputs(cfg, [0, at, 0], S, BF16, [0, 1, 0]))[1:2]
+            at += 1
+        ids.append(out)
+        assert bool(h.isfinite().all())
+    assert ids[0] == ids[1]
+
+
+@pytest.mark.gpu
+def test_pages_need_the_8_bit_format(gpu, weights):
+    with pytest.raises(RuntimeError, match="FP8"):
+        Engine(weights[0], B, K, S, kv_pages=8)
